@@ -35,7 +35,10 @@
  *  - A tkh_context owns one HIP stream, a device workspace and the status
  *    word.  It is not thread-safe; separate contexts are independent.
  *  - No operator allocates.  Device memory is allocated only by
- *    tkh_context_create and tkh_kv_create.
+ *    tkh_context_create, tkh_kv_create, tkh_session_create and
+ *    tkh_paged_create.
+ *  - The paged cache's context rows are in the storage dtype, not FP32: the
+ *    next product of a host that batches sessions reads 16-bit rows.
  */
 #ifndef TOKHIP_H
 #define TOKHIP_H
@@ -318,6 +321,152 @@ uint32_t tkh_kv_commit_batch(tkh_kv *const *kvs, const tkh_kv_frame *frames, uin
 
 /* reset_batch (src/model/window_cache.rs:342-350): offset 0, new generation. */
 uint32_t tkh_kv_reset_batch(tkh_kv *const *kvs, uint64_t count, tkh_error *err);
+
+/* ---------------- paged caches ---------------- */
+
+/* No counterpart in the reference: K and V of many sequences in one pool of
+ * pages, for hosts that serve sessions of unknown lengths or shared prefixes.
+ *
+ * Element (head h, row r, feature d) of page g of one layer's K (or V) sits at
+ * g * page_stride + h * head_stride + r * row_stride + d.  page_tokens is a
+ * power of two from 16 to 1024, head_dim 64, 128 or 256; strides are multiples
+ * of 8 elements, pointers of 16 bytes. */
+typedef struct tkh_paged_layout {
+    uint64_t pages, page_tokens, kv_heads, head_dim;
+    uint64_t page_stride, head_stride, row_stride;
+} tkh_paged_layout;
+
+/* A ragged batch over a paged cache.  The pointers are device arrays, read by
+ * each launch (and by each replay of a captured one), so lengths and tables may
+ * change between replays within the bounds given here.  Sequence b has its
+ * table row and length at slots[b] (slots NULL: at b); its new tokens are the
+ * rows query_start[b] .. query_start[b + 1] - 1 of the batch's tensors
+ * (query_start NULL: max_queries rows each, total_queries = sequences *
+ * max_queries).  key_lens counts its keys, the new tokens among them: token i of
+ * n sits at position key_lens - n + i.  Table entries past the last key are not
+ * read.  Rows of no sequence (behind the last one) are neither read nor written.
+ * A sequence whose values are out of range (a slot, a row range, more than
+ * max_queries rows or max_keys keys, a page number) is reported as
+ * TKH_INVALID_CONFIG at the next status check and reads and writes nothing
+ * outside the buffers; results are then unspecified. */
+typedef struct tkh_paged_batch {
+    uint64_t sequences, total_queries, max_queries, max_keys;
+    uint64_t table_rows, table_stride;
+    const int32_t *page_table;  /* [table_rows, table_stride] */
+    const int32_t *key_lens;    /* [table_rows] */
+    const int32_t *query_start; /* [sequences + 1], not decreasing, or NULL */
+    const int32_t *slots;       /* [sequences], or NULL */
+} tkh_paged_batch;
+
+/* Causal GQA of a batch's new tokens over their sequences' pages, which hold
+ * the new tokens' K/V already.  Query at position p sees keys j <= p, with a
+ * window p - j < window (0: none), scores scale * q.k, then softcap (0: none).
+ * A query that sees nothing (its position is below 0) gets a row of zeros.
+ * q and context: [total_queries, query_heads, head_dim] in `dtype`; the context
+ * is rounded once from FP32.  k_len/v_len: elements behind the pointers, at
+ * least the last page's end. */
+uint32_t tkh_paged_attention(tkh_context *ctx, const tkh_paged_batch *batch,
+                             const tkh_paged_layout *layout, uint64_t query_heads, tkh_dtype dtype,
+                             const void *q, uint64_t q_len, const void *k_pages, uint64_t k_len,
+                             const void *v_pages, uint64_t v_len, float scale, uint64_t window,
+                             float softcap, void *context, uint64_t context_len, tkh_error *err);
+
+/* Rotary positions of a paged producer.  Pairs of the first rotated_dims
+ * features (a multiple of 8; 0: all of the head) turn, the others pass: (j, j +
+ * rotated_dims/2), or (2j, 2j + 1) interleaved.  Pair j's frequency is
+ * theta^(-2j/rotated_dims); linear scaling divides it by factor; bands keep it
+ * where original_max_positions hold high_freq_factor or more of its rotations,
+ * divide it by factor where they hold low_freq_factor or fewer, and blend
+ * linearly in the count between (TKH_ROTARY_LLAMA3's rule).  magnitude
+ * multiplies sine and cosine (1: none). */
+typedef enum tkh_rope_layout { TKH_ROPE_NONE = 0, TKH_ROPE_HALF = 1, TKH_ROPE_INTERLEAVED = 2 } tkh_rope_layout;
+typedef enum tkh_rope_scaling { TKH_ROPE_UNSCALED = 0, TKH_ROPE_LINEAR = 1, TKH_ROPE_BANDS = 2 } tkh_rope_scaling;
+typedef struct tkh_rope {
+    uint32_t layout;  /* tkh_rope_layout */
+    uint32_t scaling; /* tkh_rope_scaling */
+    uint64_t rotated_dims;
+    float theta, factor, low_freq_factor, high_freq_factor, magnitude;
+    uint64_t original_max_positions;
+} tkh_rope;
+
+/* The step before tkh_paged_attention for every row of a batch: per-head
+ * RMSNorm of Q and K where weights are given (FP32 [head_dim] or NULL), rotary
+ * at the row's position, one rounding; Q to q_out [total_queries, query_heads,
+ * head_dim], K and V into the row's page.  Projections are token-major in
+ * proj_dtype (TKH_F32 or any storage dtype): token t's heads start t * stride
+ * elements in (strides in multiples of 4 elements, at least one token's row), so
+ * Q, K and V may be slices of one product.  No two rows of a batch may share a
+ * page row. */
+typedef struct tkh_paged_projections {
+    const void *q, *k, *v;
+    uint64_t q_stride, k_stride, v_stride;
+    uint64_t q_len, k_len, v_len;  /* elements from each pointer on */
+    const float *q_norm, *k_norm;
+    float norm_epsilon;
+} tkh_paged_projections;
+uint32_t tkh_paged_produce(tkh_context *ctx, const tkh_paged_batch *batch,
+                           const tkh_paged_layout *layout, const tkh_rope *rope,
+                           uint64_t query_heads, tkh_dtype proj_dtype,
+                           const tkh_paged_projections *proj, tkh_dtype dtype, void *q_out,
+                           uint64_t q_out_len, void *k_pages, uint64_t k_len, void *v_pages,
+                           uint64_t v_len, tkh_error *err);
+
+/* Copies page src[i] to page dst[i] in every plane (a layer's K or V), as if one
+ * after the other in order: a page may be copied on from where it was copied to.
+ * Plane l, page g starts l * plane_stride + g * page_stride bytes into the pool.
+ * src/dst are host arrays, read before the call returns. */
+uint32_t tkh_copy_pages(tkh_context *ctx, void *pool, uint64_t pool_bytes, uint64_t planes,
+                        uint64_t plane_stride, uint64_t pages, uint64_t page_stride,
+                        uint64_t page_bytes, const uint64_t *src, const uint64_t *dst,
+                        uint64_t count, tkh_error *err);
+
+/* Owner of a paged cache: the pool, the page tables and the pages' reference
+ * counts.  Its device table and lengths are what a batch's page_table and
+ * key_lens name, its sequences the slots.  Changes are queued on the context's
+ * stream, so calls queued after them see them; while that stream is being
+ * captured they are refused (TKH_UNSUPPORTED: a replay would not repeat the
+ * host's part).  ctx NULL: the bookkeeping alone, for planning and for testing
+ * without a device. */
+typedef struct tkh_paged_kv tkh_paged_kv;
+typedef struct tkh_paged_options {
+    uint64_t layers, kv_heads, head_dim, page_tokens, pages;
+    uint64_t sequences;      /* open at once */
+    uint64_t sequence_pages; /* of one sequence at most */
+    tkh_dtype storage;
+} tkh_paged_options;
+uint32_t tkh_paged_create(tkh_context *ctx, const tkh_paged_options *options, tkh_paged_kv **out,
+                          tkh_error *err);
+/* Safe in any order with tkh_context_destroy of the owning context. */
+void tkh_paged_destroy(tkh_paged_kv *kv);
+
+typedef struct tkh_paged_info {
+    uint64_t layers, kv_heads, head_dim, page_tokens, pages, sequences, sequence_pages;
+    uint64_t free_pages, open_sequences, allocated_bytes;
+    void *pool;              /* [layers, 2 (K, V), pages, kv_heads, page_tokens, head_dim] */
+    int32_t *page_table;     /* [sequences, sequence_pages] */
+    int32_t *key_lens;       /* [sequences] */
+    tkh_dtype storage;
+} tkh_paged_info;
+uint32_t tkh_paged_info_get(const tkh_paged_kv *kv, tkh_paged_info *info);
+
+/* An empty sequence, the lowest free one (TKH_CAPACITY when all are open). */
+uint32_t tkh_paged_open(tkh_paged_kv *kv, uint64_t *sequence, tkh_error *err);
+/* A new sequence with `sequence`'s keys, sharing its pages. */
+uint32_t tkh_paged_fork(tkh_paged_kv *kv, uint64_t sequence, uint64_t *forked, tkh_error *err);
+/* Room for tokens[i] more keys of sequences[i], whose lengths grow by them: new
+ * pages (the lowest free ones), and a copy of a partly filled last page that
+ * another sequence shares.  All or nothing: TKH_CAPACITY leaves everything as it
+ * was, and a sequence given twice is refused. */
+uint32_t tkh_paged_extend(tkh_paged_kv *kv, const uint64_t *sequences, const uint64_t *tokens,
+                          uint64_t count, tkh_error *err);
+/* The first `length` keys stay; pages that no sequence holds any more are freed. */
+uint32_t tkh_paged_truncate(tkh_paged_kv *kv, uint64_t sequence, uint64_t length, tkh_error *err);
+uint32_t tkh_paged_close(tkh_paged_kv *kv, uint64_t sequence, tkh_error *err);
+/* Moves the pages in use to the pool's lowest numbers (*moved: how many moved). */
+uint32_t tkh_paged_compact(tkh_paged_kv *kv, uint64_t *moved, tkh_error *err);
+/* A sequence's length and page numbers (at most `capacity` of them written). */
+uint32_t tkh_paged_sequence_get(const tkh_paged_kv *kv, uint64_t sequence, uint64_t *length,
+                                uint64_t *pages, uint64_t capacity);
 
 /* ---------------- producer (the step before attention) ---------------- */
 

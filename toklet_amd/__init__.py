@@ -14,6 +14,6 @@ def __getattr__(name):
     # Lazy submodules so `import toklet_amd` works without torch's CUDA state.
     import importlib
 
-    if name in ("ops", "kv", "session", "build"):
+    if name in ("ops", "kv", "paged", "session", "build"):
         return importlib.import_module(f".{name}", __name__)
     raise AttributeError(name)

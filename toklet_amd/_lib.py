@@ -103,6 +103,41 @@ class LayerIo(ctypes.Structure):
     _fields_ = [(n, vp) for n in ("q_proj", "k_proj", "v_proj", "q_norm", "k_norm", "context")]
 
 
+class PagedLayout(ctypes.Structure):
+    _fields_ = [(n, u64) for n in ("pages", "page_tokens", "kv_heads", "head_dim", "page_stride",
+                                   "head_stride", "row_stride")]
+
+
+class PagedBatch(ctypes.Structure):
+    _fields_ = [(n, u64) for n in ("sequences", "total_queries", "max_queries", "max_keys",
+                                   "table_rows", "table_stride")] + [
+        (n, vp) for n in ("page_table", "key_lens", "query_start", "slots")]
+
+
+class Rope(ctypes.Structure):
+    _fields_ = [("layout", u32), ("scaling", u32), ("rotated_dims", u64)] + [
+        (n, f32) for n in ("theta", "factor", "low_freq_factor", "high_freq_factor", "magnitude")] + [
+        ("original_max_positions", u64)]
+
+
+class PagedProjections(ctypes.Structure):
+    _fields_ = [(n, vp) for n in ("q", "k", "v")] + [
+        (n, u64) for n in ("q_stride", "k_stride", "v_stride", "q_len", "k_len", "v_len")] + [
+        ("q_norm", vp), ("k_norm", vp), ("norm_epsilon", f32)]
+
+
+class PagedOptions(ctypes.Structure):
+    _fields_ = [(n, u64) for n in ("layers", "kv_heads", "head_dim", "page_tokens", "pages",
+                                   "sequences", "sequence_pages")] + [("storage", ctypes.c_int)]
+
+
+class PagedInfo(ctypes.Structure):
+    _fields_ = [(n, u64) for n in ("layers", "kv_heads", "head_dim", "page_tokens", "pages",
+                                   "sequences", "sequence_pages", "free_pages", "open_sequences",
+                                   "allocated_bytes")] + [
+        (n, vp) for n in ("pool", "page_table", "key_lens")] + [("storage", ctypes.c_int)]
+
+
 P = ctypes.POINTER
 E = P(Error)
 
@@ -141,6 +176,21 @@ SIGNATURES = {
     "tkh_kv_view": (u32, [vp, P(KvFrame), u64, f32, P(Segment), P(SpanShape), E]),
     "tkh_kv_commit_batch": (u32, [P(vp), P(KvFrame), u64, E]),
     "tkh_kv_reset_batch": (u32, [P(vp), u64, E]),
+    "tkh_paged_attention": (u32, [vp, P(PagedBatch), P(PagedLayout), u64, ctypes.c_int, vp, u64, vp,
+                                  u64, vp, u64, f32, u64, f32, vp, u64, E]),
+    "tkh_paged_produce": (u32, [vp, P(PagedBatch), P(PagedLayout), P(Rope), u64, ctypes.c_int,
+                                P(PagedProjections), ctypes.c_int, vp, u64, vp, u64, vp, u64, E]),
+    "tkh_copy_pages": (u32, [vp, vp, u64, u64, u64, u64, u64, u64, vp, vp, u64, E]),
+    "tkh_paged_create": (u32, [vp, P(PagedOptions), P(vp), E]),
+    "tkh_paged_destroy": (None, [vp]),
+    "tkh_paged_info_get": (u32, [vp, P(PagedInfo)]),
+    "tkh_paged_open": (u32, [vp, P(u64), E]),
+    "tkh_paged_fork": (u32, [vp, u64, P(u64), E]),
+    "tkh_paged_extend": (u32, [vp, P(u64), P(u64), u64, E]),
+    "tkh_paged_truncate": (u32, [vp, u64, u64, E]),
+    "tkh_paged_close": (u32, [vp, u64, E]),
+    "tkh_paged_compact": (u32, [vp, P(u64), E]),
+    "tkh_paged_sequence_get": (u32, [vp, u64, P(u64), P(u64), u64]),
     "tkh_produce_qkv": (u32, [vp, P(ProducerShape), ctypes.c_int, vp, vp, vp, vp, vp, vp, vp, vp,
                               u64, E]),
     "tkh_session_create": (u32, [vp, P(SessionOptions), P(u64), P(vp), E]),

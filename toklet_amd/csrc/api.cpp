@@ -96,6 +96,9 @@ uint32_t status_error(uint32_t st, tkh_error *err) {
     if (st & tkh::ST_SPLIT_TIMEOUT)
         return fail(err, TKH_DEVICE, "decode splits", 0, 0, 0,
                     "a decode merge timed out waiting for its key splits (status 0x%x)", st);
+    if (st & tkh::ST_BAD_PAGE)
+        return fail(err, TKH_INVALID_CONFIG, "paged batch", 0, 0, 0,
+                    "a paged batch has a slot, row range, length or page number out of range (status 0x%x)", st);
     // A non-finite input anywhere decides first (the reference checks every
     // input before computing).
     if (st & tkh::ST_NONFINITE_INPUT)
@@ -1097,6 +1100,13 @@ uint32_t tkh_host::add_chunk_producer(tkh_context *ctx, ChunkBatchOfLayers *batc
     return TKH_OK;
 }
 
+uint32_t tkh_host::after_operator(tkh_context *ctx, tkh_error *err) { return after_launch(ctx, err); }
+
+uint32_t tkh_host::profile_events(tkh_context *ctx, bool combine, hipEvent_t **ev, tkh_error *err) {
+    *ev = nullptr;
+    return ctx->profiling ? profile_slot(ctx, ev, combine, err) : (uint32_t)TKH_OK;
+}
+
 // Puts the layers whose workgroups take the most keys first: workgroups start in
 // order, and a long one that starts last runs on a card that has emptied (figures
 // at pf_locate).
@@ -1200,10 +1210,12 @@ uint32_t tkh_context_create(int device, void *stream, size_t workspace_bytes, in
     // The caller's stream, or the device's null stream: work is ordered with
     // whatever the caller queued there (no private stream, no priorities).
     ctx->stream = reinterpret_cast<hipStream_t>(stream);
-    const size_t status_bytes = 256 + sizeof(uint32_t) * tkh_softcap_verdicts();
+    const size_t verdict_bytes = (sizeof(uint32_t) * tkh_softcap_verdicts() + 255) / 256 * 256;
+    const size_t status_bytes = 256 + verdict_bytes + sizeof(uint32_t) * kPagedCounters;
     if ((e = hipMalloc(&ctx->status_dev, status_bytes)) != hipSuccess) return cleanup(e, "status");
     if ((e = hipMemset(ctx->status_dev, 0, status_bytes)) != hipSuccess) return cleanup(e, "status");
     ctx->verdict_dev = ctx->status_dev + 256 / sizeof(uint32_t);
+    ctx->paged_counters = ctx->verdict_dev + verdict_bytes / sizeof(uint32_t);
     if ((e = hipHostMalloc(&ctx->status_host, sizeof(uint32_t), hipHostMallocDefault)) != hipSuccess)
         return cleanup(e, "status");
     if ((e = hipMalloc(&ctx->workspace, ctx->workspace_bytes)) != hipSuccess)

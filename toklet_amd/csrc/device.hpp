@@ -24,6 +24,7 @@ enum StatusBits : uint32_t {
     ST_SPLIT_TIMEOUT = 8u,     // a decode merge gave up waiting for the other key splits
     // 16u: unused (a value-range refusal the chunk kernel no longer makes)
     ST_NONFINITE_LOGIT = 32u,  // a projected logit is not finite (project.hip)
+    ST_BAD_PAGE = 64u,         // a paged batch names a page, length or row out of range
 };
 
 // The o-projection and greedy pick (project.hip).

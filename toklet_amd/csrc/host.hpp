@@ -16,6 +16,7 @@ namespace tkh_host {
 
 inline constexpr int kSlots = 16;
 inline constexpr int kSlotProblems = 1024;
+inline constexpr int kPagedCounters = 1 << 16;
 
 // ---------------------------------------------------------------- errors
 
@@ -147,6 +148,7 @@ struct tkh_context {
     bool decode_merge_batch = false;  // compact-batch decode: combine in a second launch
     uint32_t epoch = 0;          // last decode split-K epoch handed out (1 .. DECODE_EPOCHS)
     uint64_t split_wait_ticks = 50000000;  // bound of a decode merge's wait for its splits
+    uint32_t *paged_counters = nullptr;  // kPagedCounters arrival counters, 0 between launches, in status_dev's allocation
     bool test_flag_skew = false; // test hook: merges wait for a flag value no split stores
     int prefill_groups = 128;    // below this many row-block workgroups (128-row units), split the keys
     int prefill_fill_groups = 512;  // row-block workgroups (128-row units) from which eight-wave ones fill the device
@@ -221,6 +223,10 @@ uint32_t attention_cached_fused(tkh_context *ctx, const tkh_cached_shape *shape,
 uint32_t span_attention_fused(tkh_context *ctx, const tkh_span_shape *shape, tkh_dtype dtype,
                               const tkh_segment segments[3], float *context,
                               const tkh::FusedDecode &fused, DecodeBatchOfLayers *batch, tkh_error *err);
+// What ends every operator: a synchronous context waits and reports (api.cpp).
+uint32_t after_operator(tkh_context *ctx, tkh_error *err);
+// A launch's slot for the profile's events (null: not profiling; api.cpp).
+uint32_t profile_events(tkh_context *ctx, bool combine, hipEvent_t **ev, tkh_error *err);
 // tkh_kv_commit_batch with an optional device gate (api.cpp).
 uint32_t commit_frames(tkh_kv *const *kvs, const tkh_kv_frame *frames, uint64_t count,
                        const uint32_t *gate, uint64_t *committed, uint64_t committed_value,

@@ -1,0 +1,116 @@
+// paged.hpp - device-side types of the paged cache's kernels.
+//
+// K and V of one layer live in pages of `page_tokens` rows: element (head h,
+// row r, feature d) of page g at g * page_stride + h * head_stride +
+// r * row_stride + d.  Key j of a sequence is row j % page_tokens of page
+// table[j / page_tokens].  Tables, lengths and query ranges are device arrays
+// that a captured launch reads anew at each replay, so the kernels check every
+// value that becomes an address: a sequence that fails is skipped and
+// ST_BAD_PAGE raised.
+#pragma once
+
+#include "device.hpp"
+
+namespace tkh {
+
+struct PagedBatch {
+    const int32_t *table;        // [table_rows, table_stride]
+    const int32_t *key_lens;     // [table_rows]
+    const int32_t *query_start;  // [sequences + 1], or null: max_queries rows each
+    const int32_t *slots;        // [sequences] table rows, or null: row b
+    int64_t table_stride;
+    int32_t table_rows, sequences, max_queries, max_keys, total;
+};
+
+struct PagedLayout {
+    int64_t page_stride, head_stride, row_stride;  // elements
+    int32_t pages, page_shift;
+};
+
+struct PagedAttend {
+    PagedBatch b;
+    PagedLayout l;
+    const void *q;    // [total, Hq, D]
+    const void *k, *v;
+    void *out;        // [total, Hq, D] in the storage dtype
+    int32_t hq, hkv, group;
+    int32_t window;   // INT32_MAX: none
+    float scale_log2;
+    float softcap_y, softcap_log2;  // scale / cap and cap * log2(e); 0: no cap
+    int32_t splits;   // key splits of every (sequence, KV head, row block)
+    int32_t row_blocks;  // row blocks of the longest sequence
+    float *part_ml, *part_o;
+    uint32_t *counters;
+    uint32_t *status;
+};
+
+struct PagedRotary {
+    int32_t layout;   // 0 none, 1 half, 2 interleaved
+    int32_t rotated;  // leading features that rotate
+    int32_t scaling;  // 0 none, 1 linear, 2 bands
+    double step;      // log2 of the ratio of consecutive frequencies (negative)
+    double inv_factor, low, inv_width, original;
+    float magnitude;
+};
+
+struct PagedProduce {
+    PagedBatch b;
+    PagedLayout l;
+    PagedRotary rot;
+    const void *q, *k, *v;                // token rows of [H, D]
+    int64_t q_stride, k_stride, v_stride;  // elements between tokens
+    const float *q_norm, *k_norm;          // [D] or null
+    void *q_out;                           // [total, Hq, D]
+    void *k_pages, *v_pages;
+    int32_t hq, hkv, d;
+    float eps;
+    uint32_t *status;
+};
+
+// Page copies: pairs in the kernel's arguments, so a call uploads nothing.
+constexpr int COPY_PAGES_MAX = 480;
+struct CopyPages {
+    uint8_t *pool;
+    int64_t plane_stride, page_stride, page_bytes;  // bytes
+    int32_t planes, count;
+    uint32_t src[COPY_PAGES_MAX], dst[COPY_PAGES_MAX];
+};
+static_assert(sizeof(CopyPages) <= 4096, "kernel arguments");
+
+// Changed words of an owner's page tables and lengths, likewise.
+constexpr int PATCH_MAX = 500;
+struct PatchWords {
+    int32_t *base;
+    int32_t count;
+    uint32_t index[PATCH_MAX];
+    int32_t value[PATCH_MAX];
+};
+static_assert(sizeof(PatchWords) <= 4096, "kernel arguments");
+
+// One sequence of a batch as the kernels use it: query rows [q0, q0 + n), len
+// keys.  Anything out of range gives no rows and no keys, and `bad`.
+struct PagedSeq {
+    int32_t q0, n, len, slot;
+    bool bad;
+};
+__device__ __forceinline__ PagedSeq paged_sequence(const PagedBatch &b, int s) {
+    PagedSeq r;
+    r.slot = b.slots ? gload_ptr<int32_t>(b.slots)[s] : s;
+    int32_t q1;
+    if (b.query_start) {
+        r.q0 = gload_ptr<int32_t>(b.query_start)[s];
+        q1 = gload_ptr<int32_t>(b.query_start)[s + 1];
+    } else {
+        r.q0 = s * b.max_queries;
+        q1 = r.q0 + b.max_queries;
+    }
+    r.bad = (uint32_t)r.slot >= (uint32_t)b.table_rows || r.q0 < 0 || q1 < r.q0 || q1 > b.total ||
+            q1 - r.q0 > b.max_queries;
+    r.n = q1 - r.q0;
+    r.len = r.bad ? 0 : gload_ptr<int32_t>(b.key_lens)[r.slot];
+    r.bad |= (uint32_t)r.len > (uint32_t)b.max_keys;
+    if (r.bad) r.slot = r.q0 = r.n = r.len = 0;
+    return r;
+}
+
+}  // namespace tkh

@@ -366,3 +366,191 @@ def produce_qkv(ctx: Context, shape: ProducerShape, q_proj, k_proj, v_proj, q_no
         _ptr(v_proj), _ptr(q_norm), _ptr(k_norm), _ptr(q_out), _ptr(k_out), _ptr(v_out),
         out_head_stride, ctypes.byref(err))
     _check(rc, err)
+
+
+# ---- paged caches (no counterpart in the reference)
+
+_ROPE_LAYOUTS = {"none": 0, "half": 1, "interleaved": 2}
+_ROPE_SCALINGS = {"none": 0, "linear": 1, "bands": 2}
+
+
+@dataclass
+class PagedBatch:
+    """A ragged batch over a paged cache (tkh_paged_batch).  The tensors are int32 on
+    the device and are read by each launch: page_table [rows, columns] (rows may be
+    strided), key_lens [rows], query_start [sequences + 1] or None (max_queries rows
+    each), slots [sequences] (a sequence's table row) or None.  The integers bound
+    what the tensors may hold."""
+    page_table: torch.Tensor
+    key_lens: torch.Tensor
+    total_queries: int
+    max_queries: int
+    max_keys: int
+    query_start: Optional[torch.Tensor] = None
+    slots: Optional[torch.Tensor] = None
+
+    def _c(self, device: int):
+        for name in ("page_table", "key_lens", "query_start", "slots"):
+            t = getattr(self, name)
+            if t is None:
+                continue
+            if t.dtype is not torch.int32:
+                raise TypeError(f"{name} is an int32 tensor")
+            if t.device.type != "cuda" or t.device.index != device:
+                raise ValueError(f"{name} is not on the context's device")
+            if t.dim() != (2 if name == "page_table" else 1) or t.stride(-1) != 1 and t.shape[-1] > 1:
+                raise ValueError(f"{name} has the wrong dimensions or strides")
+        rows, columns = self.page_table.shape
+        if self.key_lens.shape[0] != rows:
+            raise ValueError("page_table and key_lens have one row per sequence slot")
+        # Rows may lie further apart than their columns, or be one broadcast row.
+        stride = self.page_table.stride(0) if rows > 1 else columns
+        if rows > 1 and stride < columns:
+            raise ValueError("page_table has the wrong dimensions or strides")
+        if self.max_keys < 1 or self.max_queries < 1 or self.total_queries < 0:
+            raise ValueError("a batch's bounds are positive")
+        if self.query_start is not None:
+            sequences = self.query_start.shape[0] - 1
+        else:
+            sequences = self.slots.shape[0] if self.slots is not None else rows
+        if self.slots is not None and self.slots.shape[0] != sequences:
+            raise ValueError("slots and query_start disagree")
+        return _lib.PagedBatch(max(sequences, 0), self.total_queries, self.max_queries, self.max_keys, rows,
+                               stride, _ptr(self.page_table), _ptr(self.key_lens),
+                               _ptr(self.query_start), _ptr(self.slots))
+
+
+@dataclass
+class RotaryPositions:
+    """Rotary positions of a paged producer (tkh_rope).  layout: "none", "half" (pairs
+    j, j + rotated_dims/2) or "interleaved" (2j, 2j + 1); rotated_dims 0: all of the
+    head; scaling: "none", "linear" (frequencies / factor) or "bands" (kept, blended or
+    divided by how many rotations original_max_positions hold); magnitude multiplies
+    sine and cosine."""
+    layout: str = "half"
+    rotated_dims: int = 0
+    theta: float = 1e6
+    scaling: str = "none"
+    factor: float = 1.0
+    low_freq_factor: float = 1.0
+    high_freq_factor: float = 4.0
+    original_max_positions: int = 8192
+    magnitude: float = 1.0
+
+    def _c(self):
+        if self.layout not in _ROPE_LAYOUTS or self.scaling not in _ROPE_SCALINGS:
+            raise ValueError(f"rotary layout {self.layout!r}, scaling {self.scaling!r}")
+        return _lib.Rope(_ROPE_LAYOUTS[self.layout], _ROPE_SCALINGS[self.scaling], self.rotated_dims,
+                         self.theta, self.factor, self.low_freq_factor, self.high_freq_factor,
+                         self.magnitude, self.original_max_positions)
+
+
+def _on_device(ctx: Context, *tensors):
+    for t in tensors:
+        if t is not None and (t.device.type != "cuda" or t.device.index != ctx.device):
+            raise ValueError("a tensor is not on the context's device")
+
+
+def _paged_layout(k_pages: torch.Tensor, v_pages: torch.Tensor):
+    """The layout of page tensors [pages, kv_heads, page_tokens, head_dim] (any strides
+    with contiguous rows) and the elements from their first on."""
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
+        raise ValueError("k_pages and v_pages are [pages, kv_heads, page_tokens, head_dim] alike")
+    if k_pages.stride(3) != 1:
+        raise ValueError("page rows are contiguous")
+    pages, heads, tokens, dims = k_pages.shape
+    ps, hs, rs, _ = k_pages.stride()
+    ps, hs = ps if pages > 1 else 0, hs if heads > 1 else 0  # torch leaves these strides open
+    extent = (pages - 1) * ps + (heads - 1) * hs + (tokens - 1) * rs + dims if k_pages.numel() else 0
+    return _lib.PagedLayout(pages, tokens, heads, dims, ps, hs, rs), extent
+
+
+def _rows(t: torch.Tensor, name: str, heads: int, dims: int):
+    """Tokens and stride of a token-major [tokens, heads, dims] tensor whose tokens are contiguous."""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dims:
+        raise ValueError(f"{name} is [tokens, {heads}, {dims}]")
+    if t.numel() and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != dims)):
+        raise ValueError(f"{name}: a token's heads are contiguous")
+    tokens = t.shape[0]
+    stride = t.stride(0) if tokens > 1 else heads * dims
+    return tokens, stride, (tokens - 1) * stride + heads * dims if tokens else 0
+
+
+def paged_attention(ctx: Context, batch: PagedBatch, q, k_pages, v_pages, context, *, scale: float,
+                    window: Optional[int] = None, softcap: float = 0.0):
+    """Causal GQA of a ragged batch's new tokens over their pages (tkh_paged_attention).
+    q/context: [total_queries, query_heads, head_dim], in the pages' dtype."""
+    dt = dtype_of(q, k_pages, v_pages, context)
+    _on_device(ctx, q, k_pages, v_pages, context)
+    layout, extent = _paged_layout(k_pages, v_pages)
+    heads = q.shape[1] if q.dim() == 3 else 0
+    if q.dim() != 3 or q.shape != context.shape or q.shape[2] != layout.head_dim:
+        raise ValueError("q and context are [total_queries, query_heads, head_dim]")
+    if not q.is_contiguous() or not context.is_contiguous():
+        raise ValueError("q and context are contiguous")
+    if window is not None and window < 1:
+        raise ValueError("window is at least 1 (None: no window)")
+    err = _lib.Error()
+    b = batch._c(ctx.device)
+    rc = _lib.load().tkh_paged_attention(
+        ctx.handle, ctypes.byref(b), ctypes.byref(layout), heads, dt, _ptr(q), _n(q), _ptr(k_pages), extent,
+        _ptr(v_pages), extent, scale, window or 0, softcap, _ptr(context), _n(context), ctypes.byref(err))
+    _check(rc, err)
+
+
+def paged_produce(ctx: Context, batch: PagedBatch, rotary: RotaryPositions, q_proj, k_proj, v_proj, q_norm,
+                  k_norm, q_out, k_pages, v_pages, norm_epsilon: float = 1e-6):
+    """RMSNorm (optional), rotary and rounding of a ragged batch's new rows: Q to q_out
+    [total_queries, query_heads, head_dim], K and V into their pages (tkh_paged_produce).
+    Projections: [total_queries, heads, head_dim] in one dtype, rows of any stride."""
+    dt = dtype_of(q_out, k_pages, v_pages)
+    src = dtype_of(q_proj, k_proj, v_proj)
+    _on_device(ctx, q_proj, k_proj, v_proj, q_norm, k_norm, q_out, k_pages, v_pages)
+    layout, extent = _paged_layout(k_pages, v_pages)
+    hkv, dims = layout.kv_heads, layout.head_dim
+    if q_out.dim() != 3 or not q_out.is_contiguous():
+        raise ValueError("q_out is contiguous [total_queries, query_heads, head_dim]")
+    hq = q_out.shape[1]
+    rows = [_rows(t, n, h, dims) for t, n, h in ((q_proj, "q_proj", hq), (k_proj, "k_proj", hkv), (v_proj, "v_proj", hkv))]
+    if any(r[0] != batch.total_queries for r in rows):
+        raise ValueError("projections hold total_queries tokens")
+    for w in (q_norm, k_norm):
+        if w is not None and (w.dtype is not torch.float32 or w.shape != (dims,) or not w.is_contiguous()):
+            raise ValueError("norm weights are float32 [head_dim]")
+    proj = _lib.PagedProjections(_ptr(q_proj), _ptr(k_proj), _ptr(v_proj), *(r[1] for r in rows),
+                                 *(r[2] for r in rows), _ptr(q_norm), _ptr(k_norm), norm_epsilon)
+    err = _lib.Error()
+    b, rope = batch._c(ctx.device), rotary._c()
+    rc = _lib.load().tkh_paged_produce(
+        ctx.handle, ctypes.byref(b), ctypes.byref(layout), ctypes.byref(rope), hq, src, ctypes.byref(proj), dt,
+        _ptr(q_out), _n(q_out), _ptr(k_pages), extent, _ptr(v_pages), extent, ctypes.byref(err))
+    _check(rc, err)
+
+
+def copy_pages(ctx: Context, pool: torch.Tensor, src, dst):
+    """pool[:, dst[i]] = pool[:, src[i]] for each i in order (tkh_copy_pages).  pool:
+    [planes, pages, ...] with contiguous pages; src/dst: integers, or int64 CPU tensors."""
+    if pool.dtype not in _DTYPES:
+        raise TypeError(f"unsupported dtype {pool.dtype}")
+    _on_device(ctx, pool)
+    if pool.dim() < 3 or pool.numel() == 0 or not pool[0, 0].is_contiguous():
+        raise ValueError("pool is [planes, pages, ...] with contiguous pages")
+    lists = []
+    for t in (src, dst):
+        if not isinstance(t, torch.Tensor):
+            t = torch.tensor(list(t), dtype=torch.int64)
+        if t.dtype is not torch.int64 or t.device.type != "cpu" or t.dim() != 1 or not t.is_contiguous():
+            raise TypeError("page lists are integers or contiguous int64 CPU tensors")
+        lists.append(t)  # a negative number is past the pool's pages as an unsigned one
+    if lists[0].shape != lists[1].shape:
+        raise ValueError("src and dst have one entry per copy")
+    planes, pages = pool.shape[:2]
+    es = pool.element_size()
+    page = pool[0, 0].numel() * es
+    page_stride = pool.stride(1) * es if pages > 1 else page
+    plane_stride = pool.stride(0) * es if planes > 1 else page
+    held = (planes - 1) * plane_stride + (pages - 1) * page_stride + page
+    err = _lib.Error()
+    rc = _lib.load().tkh_copy_pages(ctx.handle, _ptr(pool), held, planes, plane_stride, pages, page_stride, page,
+                                    _ptr(lists[0]), _ptr(lists[1]), lists[0].shape[0], ctypes.byref(err))
+    _check(rc, err)
