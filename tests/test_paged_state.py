@@ -289,11 +289,17 @@ def test_copy_refusals():
 def test_bindings_refuse_tensors():
     t = torch.zeros(2, 4, dtype=torch.int32)
     b = ops.PagedBatch(page_table=t, key_lens=t[0], total_queries=1, max_queries=1, max_keys=1)
-    with pytest.raises(ValueError):
-        b._c(0)
+    with pytest.raises(TypeError):
+        b._c(0)  # not on the device
     b.page_table = t.long()
     with pytest.raises(TypeError):
-        b._c(0)
+        b._c(-1)
+    b.page_table = t[:, ::2]
+    with pytest.raises(ValueError):
+        b._c(-1)
+    b.page_table = t[:1].expand(2, 4)
+    with pytest.raises(ValueError):
+        b._c(-1)
     with pytest.raises(ValueError):
         ops.RotaryPositions(layout="spiral")._c()
     k = torch.zeros(3, 2, 16, 64)
@@ -302,7 +308,10 @@ def test_bindings_refuse_tensors():
     with pytest.raises(ValueError):
         ops._paged_layout(k, k.transpose(2, 3))
     with pytest.raises(ValueError):
-        ops._rows(torch.zeros(3, 4, 64), "q_proj", 2, 64)
+        ops._rows(torch.zeros(3, 4, 64), 3, 2, 64)
+    with pytest.raises(ValueError):
+        ops._rows(torch.zeros(3, 4, 128)[..., ::2], 3, 4, 64)
+    assert ops._rows(torch.zeros(3, 6, 64)[:, :4], 3, 4, 64) == (384, 2 * 384 + 256)
 
 
 def test_struct_layouts_match_header():

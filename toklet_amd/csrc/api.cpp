@@ -1023,6 +1023,8 @@ void init_tuning(tkh_context *ctx, int device) {
     ctx->prefill16_groups = std::max(1, env_int("TKH_PREFILL16_GROUPS", 64));
     ctx->prefill16_waves = env_int("TKH_PREFILL16_WAVES", 4) == 8 ? 8 : 4;
     ctx->tile_groups = std::max(1, env_int("TKH_TILE_GROUPS", 2 * ctx->cus));
+    ctx->paged_decode_groups = std::max(1, env_int("TKH_PAGED_DECODE_GROUPS", 8 * ctx->cus));
+    ctx->paged_decode_blocks = std::max(1, env_int("TKH_PAGED_DECODE_BLOCKS", 32));
 }
 
 // First visible key (absolute) of a query at `position` (window_attention.rs:105-107).

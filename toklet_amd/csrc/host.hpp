@@ -149,6 +149,8 @@ struct tkh_context {
     uint32_t epoch = 0;          // last decode split-K epoch handed out (1 .. DECODE_EPOCHS)
     uint64_t split_wait_ticks = 50000000;  // bound of a decode merge's wait for its splits
     uint32_t *paged_counters = nullptr;  // kPagedCounters arrival counters, 0 between launches, in status_dev's allocation
+    int paged_decode_groups = 2048;  // paged decode: workgroups to split towards
+    int paged_decode_blocks = 32;    // ... 16-key blocks per split at least
     bool test_flag_skew = false; // test hook: merges wait for a flag value no split stores
     int prefill_groups = 128;    // below this many row-block workgroups (128-row units), split the keys
     int prefill_fill_groups = 512;  // row-block workgroups (128-row units) from which eight-wave ones fill the device

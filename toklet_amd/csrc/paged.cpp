@@ -11,7 +11,10 @@
 #include "host.hpp"
 #include "paged.hpp"
 
-extern "C" hipError_t tkh_launch_paged_attend(const tkh::PagedAttend *p, int dtype, int d, hipStream_t stream);
+extern "C" hipError_t tkh_launch_paged_decode(const tkh::PagedAttend *p, int dtype, int d, hipStream_t stream,
+                                              hipEvent_t start, hipEvent_t stop);
+extern "C" hipError_t tkh_launch_paged_rows(const tkh::PagedAttend *p, int dtype, int d, hipStream_t stream,
+                                            hipEvent_t start, hipEvent_t stop);
 extern "C" hipError_t tkh_launch_paged_produce(const tkh::PagedProduce *p, int src, int dst, hipStream_t stream);
 extern "C" hipError_t tkh_launch_copy_pages(const tkh::CopyPages *c, hipStream_t stream);
 extern "C" hipError_t tkh_launch_patch_words(const tkh::PatchWords *w, hipStream_t stream);
@@ -89,6 +92,24 @@ tkh::PagedBatch device_batch(const tkh_paged_batch &b) {
 tkh::PagedLayout device_layout(const tkh_paged_layout &l) {
     return tkh::PagedLayout{(int64_t)l.page_stride, (int64_t)l.head_stride, (int64_t)l.row_stride, (int32_t)l.pages,
                             __builtin_ctzll(l.page_tokens)};
+}
+
+// Key splits of a launch of `units` (sequence, KV head, row block) triples whose
+// partials hold p.rows rows: at least min_blocks 16-key blocks each, about
+// `target` workgroups if every sequence were as long as the longest, and as many
+// as counters and workspace allow.
+void plan_splits(const tkh_context *ctx, tkh::PagedAttend &p, int64_t units, int64_t target, int64_t min_blocks, int D) {
+    const int64_t span = std::min<int64_t>(p.b.max_keys, (int64_t)p.window + p.b.max_queries);
+    const int64_t blocks = (span + 15) / 16 + 1;
+    const int64_t slot_bytes = (int64_t)p.rows * (D + 2) * sizeof(float);
+    int64_t splits = std::min<int64_t>(target / units, blocks / min_blocks);
+    splits = std::min<int64_t>(splits, ((int64_t)split_region_bytes(ctx) - 64) / slot_bytes / units);
+    if (units > kPagedCounters || splits < 2) splits = 1;
+    p.splits = (int32_t)splits;
+    p.split_blocks = (int32_t)((blocks + splits - 1) / splits);
+    p.part_ml = reinterpret_cast<float *>(ctx->workspace);
+    p.part_o = p.part_ml + (units * splits * p.rows * 2 + 3) / 4 * 4;
+    p.counters = ctx->paged_counters;
 }
 
 // A captured replay would repeat a launch but not the host's bookkeeping.
@@ -182,10 +203,21 @@ uint32_t tkh_paged_attention(tkh_context *ctx, const tkh_paged_batch *batch, con
     p.scale_log2 = scale * 1.4426950408889634f;
     p.softcap_y = softcap != 0.0f ? scale / softcap : 0.0f;
     p.softcap_log2 = softcap * 1.4426950408889634f;
-    p.splits = 1;
     p.status = ctx->status_dev;
     HIP_TRY(hipSetDevice(ctx->device), "hipSetDevice");
-    HIP_TRY(tkh_launch_paged_attend(&p, (int)dtype, (int)layout->head_dim, ctx->stream), "paged attention launch");
+    const int D = (int)layout->head_dim;
+    const int64_t rows_each = (int64_t)p.b.max_queries * p.group;
+    hipEvent_t *ev = nullptr;
+    TRY(profile_events(ctx, false, &ev, err));
+    hipError_t e;
+    if (dtype != TKH_F32 && rows_each <= 16) {
+        p.rows = (int32_t)rows_each;
+        plan_splits(ctx, p, (int64_t)p.b.sequences * p.hkv, ctx->paged_decode_groups, ctx->paged_decode_blocks, D);
+        e = tkh_launch_paged_decode(&p, (int)dtype, D, ctx->stream, ev ? ev[0] : nullptr, ev ? ev[1] : nullptr);
+    } else {
+        e = tkh_launch_paged_rows(&p, (int)dtype, D, ctx->stream, ev ? ev[0] : nullptr, ev ? ev[1] : nullptr);
+    }
+    HIP_TRY(e, "paged attention launch");
     return after_operator(ctx, err);
 }
 

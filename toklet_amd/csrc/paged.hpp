@@ -37,10 +37,11 @@ struct PagedAttend {
     int32_t window;   // INT32_MAX: none
     float scale_log2;
     float softcap_y, softcap_log2;  // scale / cap and cap * log2(e); 0: no cap
-    int32_t splits;   // key splits of every (sequence, KV head, row block)
-    int32_t row_blocks;  // row blocks of the longest sequence
-    float *part_ml, *part_o;
-    uint32_t *counters;
+    int32_t splits;        // most key splits of a (sequence, KV head, row block)
+    int32_t split_blocks;  // 16-key blocks a split has at least
+    int32_t rows;          // packed rows (tokens x group) a partial holds
+    float *part_ml, *part_o;  // [slot, rows, 2] and [slot, rows, D]
+    uint32_t *counters;       // per (sequence, KV head, row block): splits that have arrived
     uint32_t *status;
 };
 

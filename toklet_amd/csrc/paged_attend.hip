@@ -1,14 +1,361 @@
 // paged_attend.hip - attention over a page table.
 //
+// Query i of a sequence's n new tokens, at position p = L - n + i of L keys, sees
+// keys j <= p with p - j < window; s_j = scale q.k_j (capped: c tanh(s_j / c)),
+// o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m), in one pass with a running
+// maximum m and mass.  Scores live in units of log2.
+//
+// paged_decode: up to 16 packed rows (tokens x query heads of one KV head) per
+// (sequence, KV head), 16-bit storage; bound by the bytes of K and V.
+//  * The keys are cut into blocks of 16, which never leave a page, and a
+//    workgroup takes one split of them.  Its waves take blocks in turn, each
+//    through a ring of its own in LDS filled by direct global->LDS loads: no
+//    barrier, no register waits for memory, and the page number of a block is
+//    wave-uniform, so its address is one scalar base.
+//  * S^T = K Q^T on v_mfma_f32_16x16x32 (K rows as the A operand straight from
+//    LDS), which leaves lane l with query row l % 16 and keys 4 (l / 16) + 0..3:
+//    the B operand of O^T = V^T P^T on v_mfma_f32_16x16x16, so P never moves
+//    between lanes.  V^T is read by the transposing LDS load.
+//  * Rows' maxima move only when a score passes them by 8 (a factor of 256,
+//    which FP32 sums and 16-bit weights hold).
+//  * Splits store their partial and count up an arrival counter; the last one
+//    to arrive merges all of them in split order, so the result does not depend
+//    on who is last, and leaves the counter at 0.
+//
 // paged_rows: one wave per (query row, head), FP32 throughout.
+#include <cstddef>
+#include <type_traits>
+
 #include "paged.hpp"
 
 namespace tkh {
 
-template <int DT> __device__ __forceinline__ void store_row(void *base, int64_t i, float x);
-template <> __device__ __forceinline__ void store_row<F32>(void *base, int64_t i, float x) { reinterpret_cast<float *>(base)[i] = x; }
-template <> __device__ __forceinline__ void store_row<F16>(void *base, int64_t i, float x) { reinterpret_cast<_Float16 *>(base)[i] = (_Float16)x; }
-template <> __device__ __forceinline__ void store_row<BF16>(void *base, int64_t i, float x) { reinterpret_cast<__bf16 *>(base)[i] = (__bf16)x; }
+namespace {
+
+template <class T> using lds_ptr = __attribute__((address_space(3))) T *;
+using s16x4 = short __attribute__((ext_vector_type(4)));
+using f16x4 = _Float16 __attribute__((ext_vector_type(4)));
+using bf16x4 = __bf16 __attribute__((ext_vector_type(4)));
+using u32x2 = uint32_t __attribute__((ext_vector_type(2)));
+
+template <int DT> __device__ __forceinline__ f32x4 mfma_16x16x32(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (DT == BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <int DT> __device__ __forceinline__ f32x4 mfma_16x16x16(u32x2 a, u32x2 b, f32x4 c) {
+    if constexpr (DT == BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+}
+// Four FP32 values rounded to 16 bits (to nearest even).
+template <int DT> __device__ __forceinline__ u32x2 pack4(f32x4 x) {
+    if constexpr (DT == BF16) return __builtin_bit_cast(u32x2, __builtin_convertvector(x, bf16x4));
+    else return __builtin_bit_cast(u32x2, __builtin_convertvector(x, f16x4));
+}
+template <int DT> __device__ __forceinline__ f32x4 unpack4(u32x2 w) {
+    if constexpr (DT == BF16) return __builtin_convertvector(__builtin_bit_cast(bf16x4, w), f32x4);
+    else return __builtin_convertvector(__builtin_bit_cast(f16x4, w), f32x4);
+}
+
+// Four keys of one feature: a 16-lane group reads 4 rows x 16 features of 16 bits
+// (lane j the 8 bytes of row j / 4, features 4 (j % 4)) and lane j receives
+// feature j's four rows.
+__device__ __forceinline__ u32x2 read_tr(lds_ptr<uint8_t> p) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr<s16x4>)p));
+}
+
+// 16 bytes per lane from base + off straight to LDS at m + 16 lane.  Assembly,
+// because the compiler would otherwise wait for all of them before any LDS read;
+// wait_loads orders them.  No register receives anything.
+__device__ __forceinline__ void lds_load16(const void *base, uint32_t off, uint32_t m) {
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory", "m0");
+}
+// The same for lines that are read once (marked nontemporal).
+__device__ __forceinline__ void lds_load16_once(const void *base, uint32_t off, uint32_t m) {
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "s"(m) : "memory", "m0");
+}
+// Until at most N of this wave's vector memory operations are under way.
+template <int N> __device__ __forceinline__ void wait_loads() {
+    static_assert(N < 64, "vmcnt field");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// Until this wave's LDS reads have returned: their rows may be overwritten.
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ const uint8_t *uniform_ptr(const uint8_t *p) {
+    const uint64_t x = (uint64_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+    return (const uint8_t *)(((uint64_t)hi << 32) | lo);
+}
+
+// Reductions over the lanes l, l ^ 16, l ^ 32, l ^ 48 (one query row's four lanes).
+__device__ __forceinline__ void swap_pair(float x, bool far, float &a, float &b) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto p = far ? __builtin_amdgcn_permlane32_swap(u, u, false, false) : __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t p0 = p[0], p1 = p[1];
+    a = __builtin_bit_cast(float, p0);
+    b = __builtin_bit_cast(float, p1);
+}
+__device__ __forceinline__ float quad_max(float x) {
+    float a, b;
+    swap_pair(x, false, a, b);
+    swap_pair(fmaxf(a, b), true, a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float quad_sum(float x) {
+    float a, b;
+    swap_pair(x, false, a, b);
+    swap_pair(a + b, true, a, b);
+    return a + b;
+}
+
+template <int DT> __device__ __forceinline__ void store_elem(void *base, int64_t i, float x) {
+    if constexpr (DT == F32) reinterpret_cast<float *>(base)[i] = x;
+    else if constexpr (DT == F16) reinterpret_cast<_Float16 *>(base)[i] = (_Float16)x;
+    else reinterpret_cast<__bf16 *>(base)[i] = (__bf16)x;
+}
+template <int DT> __device__ __forceinline__ void store_elem4(void *base, int64_t i, f32x4 x) {
+    if constexpr (DT == F32) *gstore_ptr<f32x4>(reinterpret_cast<float *>(base) + i) = x;
+    else *gstore_ptr<u32x2>(reinterpret_cast<uint16_t *>(base) + i) = pack4<DT>(x);
+}
+
+// Partials pass between workgroups on different XCDs: past the L2.
+__device__ __forceinline__ void shared_store(float *p, float x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float shared_load(const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// How far a score may pass the row's maximum before the maximum moves, in log2.
+constexpr float SLACK = 8.0f;
+
+}  // namespace
+
+// The ring of one wave: NS stages of one 16-key block, K rows then V rows of 2D
+// bytes.  Rows hold their 16-byte pieces permuted (piece c of row r at c ^ turn(r)),
+// so that 16 rows read at one feature fall on 16 different bank groups.
+template <int D> struct DecodeRing {
+    static constexpr int W = D == 256 ? 2 : 4;          // waves per workgroup
+    static constexpr int NS = D == 64 ? 4 : 2;          // stages per wave
+    static constexpr int row = 2 * D;
+    static constexpr int tile = 16 * row;
+    static constexpr int stage = 2 * tile;
+    static constexpr int wave_bytes = NS * stage;
+    static constexpr int bytes = W * wave_bytes;         // 64 KiB: two workgroups per CU
+    static constexpr int loads = tile / 1024;            // direct loads per tile
+    __device__ static constexpr int turn(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
+    __device__ static constexpr int at(int r, int c) { return r * row + ((c ^ turn(r)) << 4); }
+};
+
+template <int DT, int D, bool CAP>
+__global__ __launch_bounds__(64 * DecodeRing<D>::W) void paged_decode(PagedAttend p) {
+    using L = DecodeRing<D>;
+    constexpr int W = L::W, NS = L::NS, FT = D / 16, KS = D / 32;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds_mem[L::bytes];
+    __shared__ float lds_ml[W][16][2];
+    __shared__ uint32_t lds_last;
+    lds_ptr<uint8_t> lds = (lds_ptr<uint8_t>)lds_mem;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, n = lane & 15;
+    const int kvh = (int)(blockIdx.x % (uint32_t)p.hkv), split = (int)(blockIdx.x / (uint32_t)p.hkv), G = p.group;
+    const PagedSeq sq = paged_sequence(p.b, blockIdx.y);
+    if (sq.bad) {
+        raise_status(p.status, true, ST_BAD_PAGE);
+        return;
+    }
+    const int nrows = uniform(sq.n * G), pos0 = uniform(sq.len - sq.n), len = uniform(sq.len);
+    if (nrows == 0) return;
+
+    // The blocks that some row sees, and this split's share of them.
+    const int first_key = pos0 - p.window + 1 > 0 ? pos0 - p.window + 1 : 0;
+    const int b_first = first_key >> 4, b_end = (len + 15) >> 4;
+    const int blocks = b_end > b_first ? b_end - b_first : 0;
+    int active = (blocks + p.split_blocks - 1) / p.split_blocks;
+    active = active < 1 ? 1 : (active > p.splits ? p.splits : active);
+    if (split >= active) return;
+    const int per = (blocks + active - 1) / active;
+    const int b_lo = b_first + split * per;
+    const int b_hi = b_lo + per < b_end ? b_lo + per : b_end;
+    const int mine = b_hi - b_lo > wave ? (b_hi - b_lo - wave + W - 1) / W : 0;
+
+    const_ptr<int32_t> table = (const_ptr<int32_t>)(p.b.table + (int64_t)uniform(sq.slot) * p.b.table_stride);
+    const uint8_t *kb = reinterpret_cast<const uint8_t *>(p.k) + (int64_t)kvh * p.l.head_stride * 2;
+    const uint8_t *vb = reinterpret_cast<const uint8_t *>(p.v) + (int64_t)kvh * p.l.head_stride * 2;
+    const int row_bytes = (int)p.l.row_stride * 2;
+    uint32_t off[L::loads];
+    for (int i = 0; i < L::loads; ++i) {
+        const int at = i * 1024 + lane * 16, r = at / L::row, c = (at % L::row) >> 4;
+        off[i] = (uint32_t)(r * row_bytes + ((c ^ L::turn(r)) << 4));
+    }
+    const uint32_t ring = (uint32_t)uniform((int)(uintptr_t)(lds + wave * L::wave_bytes));
+    bool bad_page = false;
+    auto page_of = [&](int t) { return table[((b_lo + wave + t * W) << 4) >> p.l.page_shift]; };
+    auto issue = [&](int t, int page) {
+        const int key = (b_lo + wave + t * W) << 4;
+        if ((uint32_t)page >= (uint32_t)p.l.pages) {
+            page = 0;
+            bad_page = true;
+        }
+        const int64_t at = ((int64_t)page * p.l.page_stride + (int64_t)(key & ((1 << p.l.page_shift) - 1)) * p.l.row_stride) * 2;
+        const uint8_t *ka = uniform_ptr(kb + at), *va = uniform_ptr(vb + at);
+        const uint32_t m = ring + (uint32_t)(t % NS) * L::stage;
+        for (int i = 0; i < L::loads; ++i) lds_load16_once(ka, off[i], m + i * 1024);
+        for (int i = 0; i < L::loads; ++i) lds_load16_once(va, off[i], m + L::tile + i * 1024);
+    };
+    for (int t = 0; t < NS; ++t)
+        if (t < mine) issue(t, page_of(t));
+
+    // This lane's query row (rows past the last repeat it and see nothing).
+    const int row = n < nrows ? n : nrows - 1;
+    const int tok = row / G, head = kvh * G + row % G;
+    u32x4 q[KS];
+    for (int s = 0; s < KS; ++s)
+        q[s] = *gload_ptr<u32x4>(reinterpret_cast<const uint16_t *>(p.q) + ((int64_t)(sq.q0 + tok) * p.hq + head) * D + 32 * s + 8 * g);
+    const int pos = pos0 + tok;
+    const int lo = pos - p.window + 1, hi = n < nrows ? pos + 1 : INT32_MIN;  // visible keys [lo, hi)
+    const int all_lo = pos0 + (nrows - 1) / G - p.window + 1, all_hi = pos0 + 1;  // keys that every row sees
+
+    f32x4 acc[FT] = {};
+    float m = NEG_INF, l = 0.0f;
+    bool bad = false;
+    for (int t = 0; t < mine; ++t) {
+        // The next block's page number arrives while this one is waited for.
+        const int page_next = t + NS < mine ? page_of(t + NS) : 0;
+        // Loads of later stages may stay under way.
+        const int ahead = mine - 1 - t < NS - 1 ? mine - 1 - t : NS - 1;
+        if (NS == 4 && ahead >= 3) wait_loads<3 * 2 * L::loads>();
+        else if (NS == 4 && ahead == 2) wait_loads<2 * 2 * L::loads>();
+        else if (ahead >= 1) wait_loads<2 * L::loads>();
+        else wait_loads<0>();
+        lds_ptr<uint8_t> kt = lds + (wave * L::wave_bytes + (t % NS) * L::stage), vt = kt + L::tile;
+        const int key0 = (b_lo + wave + t * W) << 4;
+        f32x4 s = {};
+        for (int i = 0; i < KS; ++i) s = mfma_16x16x32<DT>(*(lds_ptr<u32x4>)(kt + L::at(n, g + 4 * i)), q[i], s);
+        u32x2 v[FT];
+        for (int f = 0; f < FT; ++f) {
+            const int r = 4 * g + (n >> 2);
+            v[f] = read_tr(vt + L::at(r, 2 * f + ((n & 3) >> 1)) + (n & 1) * 8);
+        }
+        float x[4];
+        for (int i = 0; i < 4; ++i) x[i] = CAP ? tanh_fast(s[i] * p.softcap_y) * p.softcap_log2 : s[i] * p.scale_log2;
+        if (key0 >= all_lo && key0 + 16 <= all_hi) {
+            for (int i = 0; i < 4; ++i) bad |= !is_finite_f(s[i]);
+        } else {
+            // Keys that this row does not see weigh nothing; the values of keys that
+            // no row sees are whatever the page holds, NaN too, and become zeros.
+            for (int i = 0; i < 4; ++i) {
+                const int key = key0 + 4 * g + i;
+                const bool seen = key >= lo && key < hi;
+                bad |= seen && !is_finite_f(s[i]);
+                x[i] = seen ? x[i] : NEG_INF;
+            }
+            uint32_t keep[2];
+            for (int i = 0; i < 2; ++i) {
+                const int key = key0 + 4 * g + 2 * i;
+                keep[i] = (key >= first_key && key < len ? 0xffffu : 0u) | (key + 1 >= first_key && key + 1 < len ? 0xffff0000u : 0u);
+            }
+            for (int f = 0; f < FT; ++f) v[f] = u32x2{v[f][0] & keep[0], v[f][1] & keep[1]};
+        }
+        const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        if (__ballot(top > m + SLACK) != 0) {
+            const float mn = fmaxf(m, quad_max(top));
+            const float c = mn == NEG_INF ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= c;
+            for (int f = 0; f < FT; ++f) acc[f] *= c;
+        }
+        const float base = m == NEG_INF ? 0.0f : m;
+        f32x4 w;
+        for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(x[i] - base);
+        const u32x2 pw = pack4<DT>(w);  // the mass is summed from the weights as rounded
+        w = unpack4<DT>(pw);
+        l += (w[0] + w[1]) + (w[2] + w[3]);
+        for (int f = 0; f < FT; ++f) acc[f] = mfma_16x16x16<DT>(v[f], pw, acc[f]);
+        if (t + NS < mine) {
+            wait_lds();
+            issue(t + NS, page_next);
+        }
+    }
+    l = quad_sum(l);
+
+    // The waves' results through LDS (each in its own ring), then one thread per
+    // four features of a row.
+    constexpr int OS = D + 4;  // floats between rows
+    static_assert(16 * OS * 4 <= L::wave_bytes, "a wave's context fits its ring");
+    wait_lds();
+    {
+        lds_ptr<float> o = (lds_ptr<float>)(lds + wave * L::wave_bytes);
+        for (int f = 0; f < FT; ++f) *(lds_ptr<f32x4>)(o + n * OS + 16 * f + 4 * g) = acc[f];
+        if (g == 0) {
+            lds_ml[wave][n][0] = m;
+            lds_ml[wave][n][1] = l;
+        }
+    }
+    raise_status(p.status, bad_page, ST_BAD_PAGE);
+    raise_status(p.status, bad, ST_NONFINITE_INPUT);
+    __syncthreads();
+    const int64_t unit = (int64_t)blockIdx.y * p.hkv + kvh, slot = unit * p.splits + split;
+    bool bad_out = false;
+    auto finish = [&](int r, int d, f32x4 o, float mass) {
+        f32x4 y = {};
+        if (pos0 + r / G >= 0)
+            for (int i = 0; i < 4; ++i) {
+                y[i] = o[i] / mass;
+                bad_out |= !is_finite_f(y[i]);
+            }
+        store_elem4<DT>(p.out, ((int64_t)(sq.q0 + r / G) * p.hq + kvh * G + r % G) * D + d, y);
+    };
+    for (int i = threadIdx.x; i < nrows * (D / 4); i += 64 * W) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float M = NEG_INF, mass = 0.0f;
+        for (int w = 0; w < W; ++w) M = fmaxf(M, lds_ml[w][r][0]);
+        const float base = M == NEG_INF ? 0.0f : M;
+        f32x4 o = {};
+        for (int w = 0; w < W; ++w) {
+            const float c = __builtin_amdgcn_exp2f(lds_ml[w][r][0] - base);
+            mass += c * lds_ml[w][r][1];
+            const f32x4 ow = *(lds_ptr<f32x4>)((lds_ptr<float>)(lds + w * L::wave_bytes) + r * OS + d);
+            for (int j = 0; j < 4; ++j) o[j] = __builtin_fmaf(c, ow[j], o[j]);
+        }
+        if (active == 1) {
+            finish(r, d, o, mass);
+        } else {
+            for (int j = 0; j < 4; ++j) shared_store(p.part_o + (slot * p.rows + r) * D + d + j, o[j]);
+            if (d == 0) {
+                shared_store(p.part_ml + (slot * p.rows + r) * 2, M);
+                shared_store(p.part_ml + (slot * p.rows + r) * 2 + 1, mass);
+            }
+        }
+    }
+    if (active > 1) {
+        __syncthreads();  // every thread's stores come before the count
+        if (threadIdx.x == 0) {
+            const uint32_t old = __hip_atomic_fetch_add(p.counters + unit, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+            lds_last = old == (uint32_t)active - 1 ? 1u : 0u;
+            if (lds_last) __hip_atomic_store(p.counters + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (!lds_last) return;
+        for (int i = threadIdx.x; i < nrows * (D / 4); i += 64 * W) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            float M = NEG_INF, mass = 0.0f;
+            f32x4 o = {};
+            for (int s = 0; s < active; ++s) {
+                const int64_t at = (unit * p.splits + s) * p.rows + r;
+                const float ms = shared_load(p.part_ml + at * 2), ls = shared_load(p.part_ml + at * 2 + 1);
+                f32x4 os;
+                for (int j = 0; j < 4; ++j) os[j] = shared_load(p.part_o + at * D + d + j);
+                const float mn = fmaxf(M, ms), base = mn == NEG_INF ? 0.0f : mn;
+                const float c0 = __builtin_amdgcn_exp2f(M - base), c1 = __builtin_amdgcn_exp2f(ms - base);
+                mass = c0 * mass + c1 * ls;
+                for (int j = 0; j < 4; ++j) o[j] = c0 * o[j] + c1 * os[j];
+                M = mn;
+            }
+            finish(r, d, o, mass);
+        }
+    }
+    raise_status(p.status, bad_out, ST_NONFINITE_OUTPUT);
+}
 
 template <int DT, int D>
 __global__ __launch_bounds__(64) void paged_rows(PagedAttend p) {
@@ -48,7 +395,7 @@ __global__ __launch_bounds__(64) void paged_rows(PagedAttend p) {
     for (int e = 0; e < E; ++e) {
         const float y = pos < 0 ? 0.0f : o[e] / l;
         bad |= !is_finite_f(y);
-        store_row<DT>(p.out, at + lane + 64 * e, y);
+        store_elem<DT>(p.out, at + lane + 64 * e, y);
     }
     raise_status(p.status, bad_page, ST_BAD_PAGE);
     raise_status(p.status, bad, ST_NONFINITE_INPUT);
@@ -56,10 +403,32 @@ __global__ __launch_bounds__(64) void paged_rows(PagedAttend p) {
 
 }  // namespace tkh
 
-extern "C" hipError_t tkh_launch_paged_attend(const tkh::PagedAttend *p, int dtype, int d, hipStream_t stream) {
+extern "C" hipError_t tkh_launch_paged_decode(const tkh::PagedAttend *p, int dtype, int d, hipStream_t stream,
+                                              hipEvent_t start, hipEvent_t stop) {
+    using namespace tkh;
+    const dim3 grid((unsigned)(p->hkv * p->splits), (unsigned)p->b.sequences);
+    auto go = [&](auto kernel, int waves) {
+        hipExtLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, stream, start, stop, 0, *p);
+        return hipGetLastError();
+    };
+    auto dims = [&](auto dt, auto cap) {
+        constexpr int DT = decltype(dt)::value;
+        constexpr bool CAP = decltype(cap)::value;
+        if (d == 64) return go(paged_decode<DT, 64, CAP>, DecodeRing<64>::W);
+        if (d == 128) return go(paged_decode<DT, 128, CAP>, DecodeRing<128>::W);
+        return go(paged_decode<DT, 256, CAP>, DecodeRing<256>::W);
+    };
+    auto caps = [&](auto dt) { return p->softcap_y != 0.0f ? dims(dt, std::true_type{}) : dims(dt, std::false_type{}); };
+    if (dtype == F16) return caps(std::integral_constant<int, F16>{});
+    if (dtype == BF16) return caps(std::integral_constant<int, BF16>{});
+    return hipErrorInvalidValue;
+}
+
+extern "C" hipError_t tkh_launch_paged_rows(const tkh::PagedAttend *p, int dtype, int d, hipStream_t stream,
+                                            hipEvent_t start, hipEvent_t stop) {
     const dim3 grid((unsigned)p->b.max_queries, (unsigned)p->hq, (unsigned)p->b.sequences), block(64);
     auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, block, 0, stream, *p);
+        hipExtLaunchKernelGGL(kernel, grid, block, 0, stream, start, stop, 0, *p);
         return hipGetLastError();
     };
     using namespace tkh;

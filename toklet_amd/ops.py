@@ -56,6 +56,9 @@ class Context:
             stream = torch.cuda.current_stream(device)
         self.device = device
         self.torch_stream = stream
+        # Where the paged operators' errors go: a fresh structure per call costs as
+        # much as the rest of the call, and a context serves one thread.
+        self.paged_error = _lib.Error()
         handle = ctypes.c_void_p()
         err = _lib.Error()
         _check(lib.tkh_context_create(device, ctypes.c_void_p(stream.cuda_stream), workspace_bytes,
@@ -390,34 +393,35 @@ class PagedBatch:
     slots: Optional[torch.Tensor] = None
 
     def _c(self, device: int):
-        for name in ("page_table", "key_lens", "query_start", "slots"):
-            t = getattr(self, name)
-            if t is None:
-                continue
-            if t.dtype is not torch.int32:
-                raise TypeError(f"{name} is an int32 tensor")
-            if t.device.type != "cuda" or t.device.index != device:
-                raise ValueError(f"{name} is not on the context's device")
-            if t.dim() != (2 if name == "page_table" else 1) or t.stride(-1) != 1 and t.shape[-1] > 1:
-                raise ValueError(f"{name} has the wrong dimensions or strides")
-        rows, columns = self.page_table.shape
-        if self.key_lens.shape[0] != rows:
+        table, lens, start, slots = self.page_table, self.key_lens, self.query_start, self.slots
+        for t in (table, lens, start, slots):
+            if t is not None and (t.dtype is not torch.int32 or t.get_device() != device):
+                raise TypeError("a batch's tensors are int32 on the context's device")
+        rows, columns = table.shape
+        # Rows may lie further apart than their columns.
+        stride, inner = table.stride()
+        if rows == 1:
+            stride = columns
+        if (inner != 1 and columns > 1) or stride < columns:
+            raise ValueError("page_table rows are contiguous and apart from each other")
+        if lens.shape != (rows,) or not lens.is_contiguous():
             raise ValueError("page_table and key_lens have one row per sequence slot")
-        # Rows may lie further apart than their columns, or be one broadcast row.
-        stride = self.page_table.stride(0) if rows > 1 else columns
-        if rows > 1 and stride < columns:
-            raise ValueError("page_table has the wrong dimensions or strides")
+        sequences = rows
+        if slots is not None:
+            if slots.dim() != 1 or not slots.is_contiguous():
+                raise ValueError("slots is contiguous [sequences]")
+            sequences = slots.shape[0]
+        if start is not None:
+            if start.dim() != 1 or not start.is_contiguous() or start.shape[0] < 1:
+                raise ValueError("query_start is contiguous [sequences + 1]")
+            if slots is not None and start.shape[0] != sequences + 1:
+                raise ValueError("slots and query_start disagree")
+            sequences = start.shape[0] - 1
         if self.max_keys < 1 or self.max_queries < 1 or self.total_queries < 0:
             raise ValueError("a batch's bounds are positive")
-        if self.query_start is not None:
-            sequences = self.query_start.shape[0] - 1
-        else:
-            sequences = self.slots.shape[0] if self.slots is not None else rows
-        if self.slots is not None and self.slots.shape[0] != sequences:
-            raise ValueError("slots and query_start disagree")
-        return _lib.PagedBatch(max(sequences, 0), self.total_queries, self.max_queries, self.max_keys, rows,
-                               stride, _ptr(self.page_table), _ptr(self.key_lens),
-                               _ptr(self.query_start), _ptr(self.slots))
+        return _lib.PagedBatch(sequences, self.total_queries, self.max_queries, self.max_keys, rows, stride,
+                               table.data_ptr(), lens.data_ptr(), None if start is None else start.data_ptr(),
+                               None if slots is None else slots.data_ptr())
 
 
 @dataclass
@@ -445,112 +449,133 @@ class RotaryPositions:
                          self.magnitude, self.original_max_positions)
 
 
-def _on_device(ctx: Context, *tensors):
-    for t in tensors:
-        if t is not None and (t.device.type != "cuda" or t.device.index != ctx.device):
+def _paged_dtype(ctx: Context, t: torch.Tensor, *others) -> int:
+    """The one dtype of tensors on the context's device."""
+    dt, device = t.dtype, ctx.device
+    if t.get_device() != device:
+        raise ValueError("a tensor is not on the context's device")
+    for x in others:
+        if x.dtype is not dt:
+            raise TypeError("the tensors share one dtype")
+        if x.get_device() != device:
             raise ValueError("a tensor is not on the context's device")
+    code = _DTYPES.get(dt)
+    if code is None:
+        raise TypeError(f"unsupported dtype {dt}")
+    return code
 
 
 def _paged_layout(k_pages: torch.Tensor, v_pages: torch.Tensor):
     """The layout of page tensors [pages, kv_heads, page_tokens, head_dim] (any strides
     with contiguous rows) and the elements from their first on."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
+    shape, strides = k_pages.shape, k_pages.stride()
+    if len(shape) != 4 or shape != v_pages.shape or strides != v_pages.stride():
         raise ValueError("k_pages and v_pages are [pages, kv_heads, page_tokens, head_dim] alike")
-    if k_pages.stride(3) != 1:
+    pages, heads, tokens, dims = shape
+    ps, hs, rs, inner = strides
+    if inner != 1:
         raise ValueError("page rows are contiguous")
-    pages, heads, tokens, dims = k_pages.shape
-    ps, hs, rs, _ = k_pages.stride()
-    ps, hs = ps if pages > 1 else 0, hs if heads > 1 else 0  # torch leaves these strides open
+    if pages == 1:  # torch leaves these strides open
+        ps = 0
+    if heads == 1:
+        hs = 0
     extent = (pages - 1) * ps + (heads - 1) * hs + (tokens - 1) * rs + dims if k_pages.numel() else 0
-    return _lib.PagedLayout(pages, tokens, heads, dims, ps, hs, rs), extent
+    return _lib.PagedLayout(pages, tokens, heads, dims, ps, hs, rs), heads, dims, extent
 
 
-def _rows(t: torch.Tensor, name: str, heads: int, dims: int):
-    """Tokens and stride of a token-major [tokens, heads, dims] tensor whose tokens are contiguous."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dims:
-        raise ValueError(f"{name} is [tokens, {heads}, {dims}]")
-    if t.numel() and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != dims)):
-        raise ValueError(f"{name}: a token's heads are contiguous")
-    tokens = t.shape[0]
-    stride = t.stride(0) if tokens > 1 else heads * dims
-    return tokens, stride, (tokens - 1) * stride + heads * dims if tokens else 0
+def _rows(t: torch.Tensor, tokens: int, heads: int, dims: int):
+    """Stride and extent of a token-major [tokens, heads, dims] tensor whose tokens are contiguous."""
+    if t.shape != (tokens, heads, dims):
+        raise ValueError(f"a projection is [{tokens}, {heads}, {dims}], not {list(t.shape)}")
+    stride, head, inner = t.stride()
+    row = heads * dims
+    if tokens <= 1:
+        stride = row
+    if tokens and (inner != 1 or (heads > 1 and head != dims)):
+        raise ValueError("a projection's token has its heads side by side")
+    return stride, (tokens - 1) * stride + row if tokens else 0
 
 
 def paged_attention(ctx: Context, batch: PagedBatch, q, k_pages, v_pages, context, *, scale: float,
                     window: Optional[int] = None, softcap: float = 0.0):
     """Causal GQA of a ragged batch's new tokens over their pages (tkh_paged_attention).
     q/context: [total_queries, query_heads, head_dim], in the pages' dtype."""
-    dt = dtype_of(q, k_pages, v_pages, context)
-    _on_device(ctx, q, k_pages, v_pages, context)
-    layout, extent = _paged_layout(k_pages, v_pages)
-    heads = q.shape[1] if q.dim() == 3 else 0
-    if q.dim() != 3 or q.shape != context.shape or q.shape[2] != layout.head_dim:
+    dt = _paged_dtype(ctx, q, k_pages, v_pages, context)
+    layout, _, dims, extent = _paged_layout(k_pages, v_pages)
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != dims or shape != context.shape:
         raise ValueError("q and context are [total_queries, query_heads, head_dim]")
     if not q.is_contiguous() or not context.is_contiguous():
         raise ValueError("q and context are contiguous")
-    if window is not None and window < 1:
+    if window is None:
+        window = 0
+    elif window < 1:
         raise ValueError("window is at least 1 (None: no window)")
-    err = _lib.Error()
-    b = batch._c(ctx.device)
+    n, err = shape[0] * shape[1] * dims, ctx.paged_error
     rc = _lib.load().tkh_paged_attention(
-        ctx.handle, ctypes.byref(b), ctypes.byref(layout), heads, dt, _ptr(q), _n(q), _ptr(k_pages), extent,
-        _ptr(v_pages), extent, scale, window or 0, softcap, _ptr(context), _n(context), ctypes.byref(err))
-    _check(rc, err)
+        ctx.handle, batch._c(ctx.device), layout, shape[1], dt, q.data_ptr(), n, k_pages.data_ptr(), extent,
+        v_pages.data_ptr(), extent, scale, window, softcap, context.data_ptr(), n, err)
+    if rc != _lib.OK:
+        raise TkhError(err)
 
 
 def paged_produce(ctx: Context, batch: PagedBatch, rotary: RotaryPositions, q_proj, k_proj, v_proj, q_norm,
                   k_norm, q_out, k_pages, v_pages, norm_epsilon: float = 1e-6):
     """RMSNorm (optional), rotary and rounding of a ragged batch's new rows: Q to q_out
     [total_queries, query_heads, head_dim], K and V into their pages (tkh_paged_produce).
-    Projections: [total_queries, heads, head_dim] in one dtype, rows of any stride."""
-    dt = dtype_of(q_out, k_pages, v_pages)
-    src = dtype_of(q_proj, k_proj, v_proj)
-    _on_device(ctx, q_proj, k_proj, v_proj, q_norm, k_norm, q_out, k_pages, v_pages)
-    layout, extent = _paged_layout(k_pages, v_pages)
-    hkv, dims = layout.kv_heads, layout.head_dim
+    Projections: [total_queries, heads, head_dim] in one dtype, tokens at any stride."""
+    dt = _paged_dtype(ctx, q_out, k_pages, v_pages)
+    src = _paged_dtype(ctx, q_proj, k_proj, v_proj)
+    layout, hkv, dims, extent = _paged_layout(k_pages, v_pages)
     if q_out.dim() != 3 or not q_out.is_contiguous():
         raise ValueError("q_out is contiguous [total_queries, query_heads, head_dim]")
-    hq = q_out.shape[1]
-    rows = [_rows(t, n, h, dims) for t, n, h in ((q_proj, "q_proj", hq), (k_proj, "k_proj", hkv), (v_proj, "v_proj", hkv))]
-    if any(r[0] != batch.total_queries for r in rows):
-        raise ValueError("projections hold total_queries tokens")
-    for w in (q_norm, k_norm):
-        if w is not None and (w.dtype is not torch.float32 or w.shape != (dims,) or not w.is_contiguous()):
-            raise ValueError("norm weights are float32 [head_dim]")
-    proj = _lib.PagedProjections(_ptr(q_proj), _ptr(k_proj), _ptr(v_proj), *(r[1] for r in rows),
-                                 *(r[2] for r in rows), _ptr(q_norm), _ptr(k_norm), norm_epsilon)
-    err = _lib.Error()
-    b, rope = batch._c(ctx.device), rotary._c()
+    tokens, hq, _ = q_out.shape
+    qs, qn = _rows(q_proj, batch.total_queries, hq, dims)
+    ks, kn = _rows(k_proj, batch.total_queries, hkv, dims)
+    vs, vn = _rows(v_proj, batch.total_queries, hkv, dims)
+    norms = [None, None]
+    for i, w in enumerate((q_norm, k_norm)):
+        if w is None:
+            continue
+        if w.dtype is not torch.float32 or w.shape != (dims,) or not w.is_contiguous() or w.get_device() != ctx.device:
+            raise ValueError("norm weights are float32 [head_dim] on the context's device")
+        norms[i] = w.data_ptr()
+    proj = _lib.PagedProjections(q_proj.data_ptr(), k_proj.data_ptr(), v_proj.data_ptr(), qs, ks, vs, qn, kn, vn,
+                                 norms[0], norms[1], norm_epsilon)
+    err = ctx.paged_error
     rc = _lib.load().tkh_paged_produce(
-        ctx.handle, ctypes.byref(b), ctypes.byref(layout), ctypes.byref(rope), hq, src, ctypes.byref(proj), dt,
-        _ptr(q_out), _n(q_out), _ptr(k_pages), extent, _ptr(v_pages), extent, ctypes.byref(err))
-    _check(rc, err)
+        ctx.handle, batch._c(ctx.device), layout, rotary._c(), hq, src, proj, dt, q_out.data_ptr(), tokens * hq * dims,
+        k_pages.data_ptr(), extent, v_pages.data_ptr(), extent, err)
+    if rc != _lib.OK:
+        raise TkhError(err)
 
 
 def copy_pages(ctx: Context, pool: torch.Tensor, src, dst):
     """pool[:, dst[i]] = pool[:, src[i]] for each i in order (tkh_copy_pages).  pool:
     [planes, pages, ...] with contiguous pages; src/dst: integers, or int64 CPU tensors."""
-    if pool.dtype not in _DTYPES:
-        raise TypeError(f"unsupported dtype {pool.dtype}")
-    _on_device(ctx, pool)
+    _paged_dtype(ctx, pool)
     if pool.dim() < 3 or pool.numel() == 0 or not pool[0, 0].is_contiguous():
         raise ValueError("pool is [planes, pages, ...] with contiguous pages")
     lists = []
     for t in (src, dst):
         if not isinstance(t, torch.Tensor):
             t = torch.tensor(list(t), dtype=torch.int64)
-        if t.dtype is not torch.int64 or t.device.type != "cpu" or t.dim() != 1 or not t.is_contiguous():
+        if t.dtype is not torch.int64 or t.get_device() != -1 or t.dim() != 1 or not t.is_contiguous():
             raise TypeError("page lists are integers or contiguous int64 CPU tensors")
         lists.append(t)  # a negative number is past the pool's pages as an unsigned one
-    if lists[0].shape != lists[1].shape:
+    src, dst = lists
+    count = src.shape[0]
+    if dst.shape[0] != count:
         raise ValueError("src and dst have one entry per copy")
-    planes, pages = pool.shape[:2]
     es = pool.element_size()
-    page = pool[0, 0].numel() * es
-    page_stride = pool.stride(1) * es if pages > 1 else page
-    plane_stride = pool.stride(0) * es if planes > 1 else page
+    shape, strides = pool.shape, pool.stride()
+    planes, pages = shape[:2]
+    page = shape[2:].numel() * es
+    page_stride = strides[1] * es if pages > 1 else page
+    plane_stride = strides[0] * es if planes > 1 else page
     held = (planes - 1) * plane_stride + (pages - 1) * page_stride + page
-    err = _lib.Error()
-    rc = _lib.load().tkh_copy_pages(ctx.handle, _ptr(pool), held, planes, plane_stride, pages, page_stride, page,
-                                    _ptr(lists[0]), _ptr(lists[1]), lists[0].shape[0], ctypes.byref(err))
-    _check(rc, err)
+    err = ctx.paged_error
+    rc = _lib.load().tkh_copy_pages(ctx.handle, pool.data_ptr(), held, planes, plane_stride, pages, page_stride, page,
+                                    src.data_ptr(), dst.data_ptr(), count, err)
+    if rc != _lib.OK:
+        raise TkhError(err)
