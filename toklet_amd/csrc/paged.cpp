@@ -104,6 +104,7 @@ void plan_splits(const tkh_context *ctx, tkh::PagedAttend &p, int64_t units, int
     const int64_t slot_bytes = (int64_t)p.rows * (D + 2) * sizeof(float);
     int64_t splits = std::min<int64_t>(target / units, blocks / min_blocks);
     splits = std::min<int64_t>(splits, ((int64_t)split_region_bytes(ctx) - 64) / slot_bytes / units);
+    splits = std::min<int64_t>(splits, tkh::PAGED_PAIRS_MAX / p.rows);
     if (units > kPagedCounters || splits < 2) splits = 1;
     p.splits = (int32_t)splits;
     p.split_blocks = (int32_t)((blocks + splits - 1) / splits);

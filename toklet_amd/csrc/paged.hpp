@@ -27,6 +27,9 @@ struct PagedLayout {
     int32_t pages, page_shift;
 };
 
+// Rows x splits whose (maximum, mass) pairs the merging workgroup holds in LDS.
+constexpr int PAGED_PAIRS_MAX = 2048;
+
 struct PagedAttend {
     PagedBatch b;
     PagedLayout l;
@@ -94,22 +97,24 @@ struct PagedSeq {
     int32_t q0, n, len, slot;
     bool bad;
 };
+// The loads are scalar, and independent of one another as far as they can be: a
+// workgroup waits for them before anything else.
 __device__ __forceinline__ PagedSeq paged_sequence(const PagedBatch &b, int s) {
     PagedSeq r;
-    r.slot = b.slots ? gload_ptr<int32_t>(b.slots)[s] : s;
     int32_t q1;
     if (b.query_start) {
-        r.q0 = gload_ptr<int32_t>(b.query_start)[s];
-        q1 = gload_ptr<int32_t>(b.query_start)[s + 1];
+        const_ptr<int32_t> start = (const_ptr<int32_t>)b.query_start + s;
+        r.q0 = start[0];
+        q1 = start[1];
     } else {
         r.q0 = s * b.max_queries;
         q1 = r.q0 + b.max_queries;
     }
-    r.bad = (uint32_t)r.slot >= (uint32_t)b.table_rows || r.q0 < 0 || q1 < r.q0 || q1 > b.total ||
-            q1 - r.q0 > b.max_queries;
+    r.slot = b.slots ? ((const_ptr<int32_t>)b.slots)[s] : s;
+    const bool no_slot = (uint32_t)r.slot >= (uint32_t)b.table_rows;
+    r.len = ((const_ptr<int32_t>)b.key_lens)[no_slot ? 0 : r.slot];
     r.n = q1 - r.q0;
-    r.len = r.bad ? 0 : gload_ptr<int32_t>(b.key_lens)[r.slot];
-    r.bad |= (uint32_t)r.len > (uint32_t)b.max_keys;
+    r.bad = no_slot || r.q0 < 0 || q1 < r.q0 || q1 > b.total || r.n > b.max_queries || (uint32_t)r.len > (uint32_t)b.max_keys;
     if (r.bad) r.slot = r.q0 = r.n = r.len = 0;
     return r;
 }

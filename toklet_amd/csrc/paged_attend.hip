@@ -123,9 +123,18 @@ template <int DT> __device__ __forceinline__ void store_elem4(void *base, int64_
     else *gstore_ptr<u32x2>(reinterpret_cast<uint16_t *>(base) + i) = pack4<DT>(x);
 }
 
-// Partials pass between workgroups on different XCDs: past the L2.
+// Partials pass between workgroups on different XCDs: these go past the L2, so a
+// store that has been acknowledged (wait_loads<0>) is there for every other
+// workgroup's load.  That orders a partial before its arrival count without an
+// agent-scope release and acquire, which write back and invalidate the XCD's
+// whole L2: with them each workgroup of a streaming launch took 28 us longer (4
+// sessions of 100k..131k keys in 4096 workgroups 512 us, in 2048 399 us).
 __device__ __forceinline__ void shared_store(float *p, float x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ float shared_load(const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+constexpr int CPOL_SC1 = 16;  // a buffer load past the L2, as shared_load
+// LDS for that many (maximum, mass) pairs.
+__device__ constexpr int pairs_bytes(int pairs) { return (pairs * 8 + 15) / 16 * 16; }
 
 // How far a score may pass the row's maximum before the maximum moves, in log2.
 constexpr float SLACK = 8.0f;
@@ -135,9 +144,15 @@ constexpr float SLACK = 8.0f;
 // The ring of one wave: NS stages of one 16-key block, K rows then V rows of 2D
 // bytes.  Rows hold their 16-byte pieces permuted (piece c of row r at c ^ turn(r)),
 // so that 16 rows read at one feature fall on 16 different bank groups.
+#ifndef PDW
+#define PDW 4
+#endif
+#ifndef PDN
+#define PDN (D == 64 ? 4 : 2)
+#endif
 template <int D> struct DecodeRing {
-    static constexpr int W = D == 256 ? 2 : 4;          // waves per workgroup
-    static constexpr int NS = D == 64 ? 4 : 2;          // stages per wave
+    static constexpr int W = PDW;          // waves per workgroup
+    static constexpr int NS = PDN;          // stages per wave
     static constexpr int row = 2 * D;
     static constexpr int tile = 16 * row;
     static constexpr int stage = 2 * tile;
@@ -154,6 +169,7 @@ __global__ __launch_bounds__(64 * DecodeRing<D>::W) void paged_decode(PagedAtten
     constexpr int W = L::W, NS = L::NS, FT = D / 16, KS = D / 32;
     __shared__ __attribute__((aligned(1024))) uint8_t lds_mem[L::bytes];
     __shared__ float lds_ml[W][16][2];
+    __shared__ float lds_mass[64 * W];
     __shared__ uint32_t lds_last;
     lds_ptr<uint8_t> lds = (lds_ptr<uint8_t>)lds_mem;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, n = lane & 15;
@@ -202,8 +218,10 @@ __global__ __launch_bounds__(64 * DecodeRing<D>::W) void paged_decode(PagedAtten
         for (int i = 0; i < L::loads; ++i) lds_load16_once(ka, off[i], m + i * 1024);
         for (int i = 0; i < L::loads; ++i) lds_load16_once(va, off[i], m + L::tile + i * 1024);
     };
+    int pages[NS];
+    for (int t = 0; t < NS; ++t) pages[t] = t < mine ? page_of(t) : 0;
     for (int t = 0; t < NS; ++t)
-        if (t < mine) issue(t, page_of(t));
+        if (t < mine) issue(t, pages[t]);
 
     // This lane's query row (rows past the last repeat it and see nothing).
     const int row = n < nrows ? n : nrows - 1;
@@ -223,8 +241,8 @@ __global__ __launch_bounds__(64 * DecodeRing<D>::W) void paged_decode(PagedAtten
         const int page_next = t + NS < mine ? page_of(t + NS) : 0;
         // Loads of later stages may stay under way.
         const int ahead = mine - 1 - t < NS - 1 ? mine - 1 - t : NS - 1;
-        if (NS == 4 && ahead >= 3) wait_loads<3 * 2 * L::loads>();
-        else if (NS == 4 && ahead == 2) wait_loads<2 * 2 * L::loads>();
+        if (NS >= 4 && ahead >= 3) wait_loads<3 * 2 * L::loads>();
+        else if (NS >= 3 && ahead == 2) wait_loads<2 * 2 * L::loads>();
         else if (ahead >= 1) wait_loads<2 * L::loads>();
         else wait_loads<0>();
         lds_ptr<uint8_t> kt = lds + (wave * L::wave_bytes + (t % NS) * L::stage), vt = kt + L::tile;
@@ -295,6 +313,7 @@ __global__ __launch_bounds__(64 * DecodeRing<D>::W) void paged_decode(PagedAtten
     raise_status(p.status, bad, ST_NONFINITE_INPUT);
     __syncthreads();
     const int64_t unit = (int64_t)blockIdx.y * p.hkv + kvh, slot = unit * p.splits + split;
+    const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(p.part_o + slot * p.rows * D, 0, 0x7FFFFFFF, 0x00020000);
     bool bad_out = false;
     auto finish = [&](int r, int d, f32x4 o, float mass) {
         f32x4 y = {};
@@ -320,7 +339,7 @@ __global__ __launch_bounds__(64 * DecodeRing<D>::W) void paged_decode(PagedAtten
         if (active == 1) {
             finish(r, d, o, mass);
         } else {
-            for (int j = 0; j < 4; ++j) shared_store(p.part_o + (slot * p.rows + r) * D + d + j, o[j]);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), to, (uint32_t)(r * D + d) * 4u, 0, CPOL_SC1);
             if (d == 0) {
                 shared_store(p.part_ml + (slot * p.rows + r) * 2, M);
                 shared_store(p.part_ml + (slot * p.rows + r) * 2 + 1, mass);
@@ -328,30 +347,65 @@ __global__ __launch_bounds__(64 * DecodeRing<D>::W) void paged_decode(PagedAtten
         }
     }
     if (active > 1) {
+        wait_loads<0>();
         __syncthreads();  // every thread's stores come before the count
         if (threadIdx.x == 0) {
-            const uint32_t old = __hip_atomic_fetch_add(p.counters + unit, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+            const uint32_t old = __hip_atomic_fetch_add(p.counters + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             lds_last = old == (uint32_t)active - 1 ? 1u : 0u;
             if (lds_last) __hip_atomic_store(p.counters + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
         __syncthreads();
         if (!lds_last) return;
-        for (int i = threadIdx.x; i < nrows * (D / 4); i += 64 * W) {
-            const int r = i / (D / 4), d = i % (D / 4) * 4;
+        // Every (maximum, mass) pair at once, into LDS; then each thread sums four
+        // features of a row over its share of the splits, several loads under way.
+        lds_ptr<f32x2> ml = (lds_ptr<f32x2>)lds;
+        const int pairs = nrows * active, items = nrows * (D / 4);
+        const float *part_ml = p.part_ml + unit * p.splits * p.rows * 2, *part_o = p.part_o + unit * p.splits * p.rows * D;
+        for (int i = threadIdx.x; i < pairs; i += 64 * W) {
+            const int s = i / nrows, r = i % nrows;
+            ml[i] = f32x2{shared_load(part_ml + (s * p.rows + r) * 2), shared_load(part_ml + (s * p.rows + r) * 2 + 1)};
+        }
+        __syncthreads();
+        const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(part_o), 0, 0x7FFFFFFF, 0x00020000);
+        // Threads share an item's splits when there are fewer items than threads.
+        const int shares = items >= 64 * W ? 1 : 64 * W / items;
+        lds_ptr<f32x4> sums = (lds_ptr<f32x4>)(lds + pairs_bytes(pairs));
+        for (int i0 = threadIdx.x; i0 < items * shares; i0 += 64 * W) {
+            const int i = i0 % items, share = i0 / items, r = i / (D / 4), d = i % (D / 4) * 4;
             float M = NEG_INF, mass = 0.0f;
+            for (int s = 0; s < active; ++s) M = fmaxf(M, ml[s * nrows + r][0]);
+            const float base = M == NEG_INF ? 0.0f : M;
             f32x4 o = {};
-            for (int s = 0; s < active; ++s) {
-                const int64_t at = (unit * p.splits + s) * p.rows + r;
-                const float ms = shared_load(p.part_ml + at * 2), ls = shared_load(p.part_ml + at * 2 + 1);
-                f32x4 os;
-                for (int j = 0; j < 4; ++j) os[j] = shared_load(p.part_o + at * D + d + j);
-                const float mn = fmaxf(M, ms), base = mn == NEG_INF ? 0.0f : mn;
-                const float c0 = __builtin_amdgcn_exp2f(M - base), c1 = __builtin_amdgcn_exp2f(ms - base);
-                mass = c0 * mass + c1 * ls;
-                for (int j = 0; j < 4; ++j) o[j] = c0 * o[j] + c1 * os[j];
-                M = mn;
+            constexpr int U = 8;
+            for (int s0 = share; s0 < active; s0 += U * shares) {
+                f32x4 part[U];
+                for (int u = 0; u < U; ++u) {
+                    const int s = s0 + u * shares;
+                    // Past the last split: out of the buffer's range, which reads as 0.
+                    const uint32_t at = s < active ? (uint32_t)((s * p.rows + r) * D + d) * 4u : 0x80000000u;
+                    part[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, CPOL_SC1));
+                }
+                for (int u = 0; u < U; ++u) {
+                    const int s = s0 + u * shares;
+                    const float c = s < active ? __builtin_amdgcn_exp2f(ml[s * nrows + r][0] - base) : 0.0f;
+                    for (int j = 0; j < 4; ++j) o[j] = __builtin_fmaf(c, part[u][j], o[j]);
+                }
             }
-            finish(r, d, o, mass);
+            for (int s = 0; s < active; ++s) mass = __builtin_fmaf(__builtin_amdgcn_exp2f(ml[s * nrows + r][0] - base), ml[s * nrows + r][1], mass);
+            if (shares == 1) {
+                finish(r, d, o, mass);
+            } else {
+                sums[i0] = o;
+                lds_mass[i0] = mass;
+            }
+        }
+        if (shares > 1) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < items; i += 64 * W) {
+                f32x4 o = sums[i];
+                for (int share = 1; share < shares; ++share) o += sums[share * items + i];
+                finish(i / (D / 4), i % (D / 4) * 4, o, lds_mass[i]);
+            }
         }
     }
     raise_status(p.status, bad_out, ST_NONFINITE_OUTPUT);
