@@ -13,6 +13,11 @@
 
 extern "C" hipError_t tkh_launch_paged_decode(const tkh::PagedAttend *p, int dtype, int d, hipStream_t stream,
                                               hipEvent_t start, hipEvent_t stop);
+extern "C" int tkh_paged_chunk_blocks(int d);
+extern "C" hipError_t tkh_launch_paged_chunk(const tkh::PagedAttend *p, int dtype, int d, int blocks, int row_blocks,
+                                             hipStream_t stream, hipEvent_t start, hipEvent_t stop);
+extern "C" hipError_t tkh_launch_paged_chunk_merge(const tkh::PagedAttend *p, int dtype, int d, int blocks, int row_blocks,
+                                                   hipStream_t stream, hipEvent_t start, hipEvent_t stop);
 extern "C" hipError_t tkh_launch_paged_rows(const tkh::PagedAttend *p, int dtype, int d, hipStream_t stream,
                                             hipEvent_t start, hipEvent_t stop);
 extern "C" hipError_t tkh_launch_paged_produce(const tkh::PagedProduce *p, int src, int dst, hipStream_t stream);
@@ -95,22 +100,56 @@ tkh::PagedLayout device_layout(const tkh_paged_layout &l) {
 }
 
 // Key splits of a launch of `units` (sequence, KV head, row block) triples whose
-// partials hold p.rows rows: at least min_blocks 16-key blocks each, about
-// `target` workgroups if every sequence were as long as the longest, and as many
-// as counters and workspace allow.
-void plan_splits(const tkh_context *ctx, tkh::PagedAttend &p, int64_t units, int64_t target, int64_t min_blocks, int D) {
+// partials hold p.rows rows: at least min_blocks blocks of `block` keys each, about
+// `target` workgroups if every sequence were as long as the longest, and at most
+// `most` (and what the workspace holds).
+void plan_splits(const tkh_context *ctx, tkh::PagedAttend &p, int64_t units, int64_t target, int64_t block,
+                 int64_t min_blocks, int64_t most, int D) {
     const int64_t span = std::min<int64_t>(p.b.max_keys, (int64_t)p.window + p.b.max_queries);
-    const int64_t blocks = (span + 15) / 16 + 1;
+    const int64_t blocks = (span + block - 1) / block + 1;
     const int64_t slot_bytes = (int64_t)p.rows * (D + 2) * sizeof(float);
     int64_t splits = std::min<int64_t>(target / units, blocks / min_blocks);
     splits = std::min<int64_t>(splits, ((int64_t)split_region_bytes(ctx) - 64) / slot_bytes / units);
-    splits = std::min<int64_t>(splits, tkh::PAGED_PAIRS_MAX / p.rows);
-    if (units > kPagedCounters || splits < 2) splits = 1;
+    splits = std::max<int64_t>(1, std::min<int64_t>(splits, most));
     p.splits = (int32_t)splits;
     p.split_blocks = (int32_t)((blocks + splits - 1) / splits);
     p.part_ml = reinterpret_cast<float *>(ctx->workspace);
     p.part_o = p.part_ml + (units * splits * p.rows * 2 + 3) / 4 * 4;
     p.counters = ctx->paged_counters;
+}
+
+// Sequences of at most 16 packed rows: paged_decode.
+uint32_t launch_decode(tkh_context *ctx, tkh::PagedAttend p, tkh_dtype dtype, int D, tkh_error *err) {
+    const int64_t units = (int64_t)p.b.sequences * p.hkv;
+    p.rows = (int32_t)std::min<int64_t>((int64_t)p.b.max_queries * p.group, p.decode_rows);
+    plan_splits(ctx, p, units, ctx->paged_decode_groups, 16, ctx->paged_decode_blocks,
+                units > kPagedCounters ? 1 : tkh::PAGED_PAIRS_MAX / p.rows, D);
+    hipEvent_t *ev = nullptr;
+    TRY(profile_events(ctx, false, &ev, err));
+    HIP_TRY(tkh_launch_paged_decode(&p, (int)dtype, D, ctx->stream, ev ? ev[0] : nullptr, ev ? ev[1] : nullptr), "paged decode launch");
+    return TKH_OK;
+}
+
+// Sequences of more: the chunk kernel, and where keys are split the merge.
+uint32_t launch_chunk(tkh_context *ctx, tkh::PagedAttend p, tkh_dtype dtype, int D, tkh_error *err) {
+    const int64_t rows_each = (int64_t)p.b.max_queries * p.group, units = (int64_t)p.b.sequences * p.hkv;
+    // Two blocks of 32 rows per wave where the row blocks then still fill the CUs.
+    int blocks = tkh_paged_chunk_blocks(D);
+    if (blocks == 2 && p.hkv * ((int64_t)p.b.total * p.group / 256) < ctx->paged_wide_groups) blocks = 1;
+    const int64_t rows = 128 * blocks, row_blocks = (rows_each + rows - 1) / rows;
+    if (units * row_blocks * 64 > INT32_MAX) return unsupported("paged batch size", err);
+    p.rows = (int32_t)rows;
+    // The rows that there can be, not what every sequence might have.
+    const int64_t likely = std::max<int64_t>(1, p.hkv * (((int64_t)p.b.total * p.group + rows - 1) / rows));
+    plan_splits(ctx, p, units * row_blocks, ctx->paged_chunk_groups * units * row_blocks / likely, 32, ctx->paged_chunk_tiles, 32, D);
+    hipEvent_t *ev = nullptr;
+    TRY(profile_events(ctx, p.splits > 1, &ev, err));
+    HIP_TRY(tkh_launch_paged_chunk(&p, (int)dtype, D, blocks, (int)row_blocks, ctx->stream, ev ? ev[0] : nullptr, ev ? ev[1] : nullptr),
+            "paged chunk launch");
+    if (p.splits > 1)
+        HIP_TRY(tkh_launch_paged_chunk_merge(&p, (int)dtype, D, blocks, (int)row_blocks, ctx->stream, ev ? ev[2] : nullptr, ev ? ev[3] : nullptr),
+                "paged merge launch");
+    return TKH_OK;
 }
 
 // A captured replay would repeat a launch but not the host's bookkeeping.
@@ -200,25 +239,23 @@ uint32_t tkh_paged_attention(tkh_context *ctx, const tkh_paged_batch *batch, con
     p.hq = (int32_t)query_heads;
     p.hkv = (int32_t)layout->kv_heads;
     p.group = p.hq / p.hkv;
-    p.window = window == 0 || window > INT32_MAX ? INT32_MAX : (int32_t)window;
+    p.window = window == 0 || window > (1u << 30) ? 1 << 30 : (int32_t)window;  // no key is further back
     p.scale_log2 = scale * 1.4426950408889634f;
     p.softcap_y = softcap != 0.0f ? scale / softcap : 0.0f;
     p.softcap_log2 = softcap * 1.4426950408889634f;
     p.status = ctx->status_dev;
     HIP_TRY(hipSetDevice(ctx->device), "hipSetDevice");
     const int D = (int)layout->head_dim;
-    const int64_t rows_each = (int64_t)p.b.max_queries * p.group;
-    hipEvent_t *ev = nullptr;
-    TRY(profile_events(ctx, false, &ev, err));
-    hipError_t e;
-    if (dtype != TKH_F32 && rows_each <= 16) {
-        p.rows = (int32_t)rows_each;
-        plan_splits(ctx, p, (int64_t)p.b.sequences * p.hkv, ctx->paged_decode_groups, ctx->paged_decode_blocks, D);
-        e = tkh_launch_paged_decode(&p, (int)dtype, D, ctx->stream, ev ? ev[0] : nullptr, ev ? ev[1] : nullptr);
-    } else {
-        e = tkh_launch_paged_rows(&p, (int)dtype, D, ctx->stream, ev ? ev[0] : nullptr, ev ? ev[1] : nullptr);
+    if (dtype == TKH_F32) {
+        hipEvent_t *ev = nullptr;
+        TRY(profile_events(ctx, false, &ev, err));
+        HIP_TRY(tkh_launch_paged_rows(&p, (int)dtype, D, ctx->stream, ev ? ev[0] : nullptr, ev ? ev[1] : nullptr), "paged attention launch");
+        return after_operator(ctx, err);
     }
-    HIP_TRY(e, "paged attention launch");
+    // A batch may have both kinds of sequences: each kernel passes the other's by.
+    p.decode_rows = 16;
+    if (p.group <= 16) TRY(launch_decode(ctx, p, dtype, D, err));
+    if ((int64_t)p.b.max_queries * p.group > 16) TRY(launch_chunk(ctx, p, dtype, D, err));
     return after_operator(ctx, err);
 }
 

@@ -37,11 +37,12 @@ struct PagedAttend {
     const void *k, *v;
     void *out;        // [total, Hq, D] in the storage dtype
     int32_t hq, hkv, group;
-    int32_t window;   // INT32_MAX: none
+    int32_t window;   // at most 2^30, which hides no key
     float scale_log2;
     float softcap_y, softcap_log2;  // scale / cap and cap * log2(e); 0: no cap
     int32_t splits;        // most key splits of a (sequence, KV head, row block)
-    int32_t split_blocks;  // 16-key blocks a split has at least
+    int32_t split_blocks;  // key blocks (16 keys; 32 for chunks) a split has at least
+    int32_t decode_rows;   // sequences of at most this many packed rows are paged_decode's, others the chunk kernel's
     int32_t rows;          // packed rows (tokens x group) a partial holds
     float *part_ml, *part_o;  // [slot, rows, 2] and [slot, rows, D]
     uint32_t *counters;       // per (sequence, KV head, row block): splits that have arrived

@@ -26,133 +26,16 @@
 #include <cstddef>
 #include <type_traits>
 
-#include "paged.hpp"
+#include "paged_device.hpp"
 
 namespace tkh {
-
-namespace {
-
-template <class T> using lds_ptr = __attribute__((address_space(3))) T *;
-using s16x4 = short __attribute__((ext_vector_type(4)));
-using f16x4 = _Float16 __attribute__((ext_vector_type(4)));
-using bf16x4 = __bf16 __attribute__((ext_vector_type(4)));
-using u32x2 = uint32_t __attribute__((ext_vector_type(2)));
-
-template <int DT> __device__ __forceinline__ f32x4 mfma_16x16x32(u32x4 a, u32x4 b, f32x4 c) {
-    if constexpr (DT == BF16)
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-template <int DT> __device__ __forceinline__ f32x4 mfma_16x16x16(u32x2 a, u32x2 b, f32x4 c) {
-    if constexpr (DT == BF16)
-        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
-}
-// Four FP32 values rounded to 16 bits (to nearest even).
-template <int DT> __device__ __forceinline__ u32x2 pack4(f32x4 x) {
-    if constexpr (DT == BF16) return __builtin_bit_cast(u32x2, __builtin_convertvector(x, bf16x4));
-    else return __builtin_bit_cast(u32x2, __builtin_convertvector(x, f16x4));
-}
-template <int DT> __device__ __forceinline__ f32x4 unpack4(u32x2 w) {
-    if constexpr (DT == BF16) return __builtin_convertvector(__builtin_bit_cast(bf16x4, w), f32x4);
-    else return __builtin_convertvector(__builtin_bit_cast(f16x4, w), f32x4);
-}
-
-// Four keys of one feature: a 16-lane group reads 4 rows x 16 features of 16 bits
-// (lane j the 8 bytes of row j / 4, features 4 (j % 4)) and lane j receives
-// feature j's four rows.
-__device__ __forceinline__ u32x2 read_tr(lds_ptr<uint8_t> p) {
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr<s16x4>)p));
-}
-
-// 16 bytes per lane from base + off straight to LDS at m + 16 lane.  Assembly,
-// because the compiler would otherwise wait for all of them before any LDS read;
-// wait_loads orders them.  No register receives anything.
-__device__ __forceinline__ void lds_load16(const void *base, uint32_t off, uint32_t m) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory", "m0");
-}
-// The same for lines that are read once (marked nontemporal).
-__device__ __forceinline__ void lds_load16_once(const void *base, uint32_t off, uint32_t m) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "s"(m) : "memory", "m0");
-}
-// Until at most N of this wave's vector memory operations are under way.
-template <int N> __device__ __forceinline__ void wait_loads() {
-    static_assert(N < 64, "vmcnt field");
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-// Until this wave's LDS reads have returned: their rows may be overwritten.
-__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ const uint8_t *uniform_ptr(const uint8_t *p) {
-    const uint64_t x = (uint64_t)p;
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
-    return (const uint8_t *)(((uint64_t)hi << 32) | lo);
-}
-
-// Reductions over the lanes l, l ^ 16, l ^ 32, l ^ 48 (one query row's four lanes).
-__device__ __forceinline__ void swap_pair(float x, bool far, float &a, float &b) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, x);
-    const auto p = far ? __builtin_amdgcn_permlane32_swap(u, u, false, false) : __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const uint32_t p0 = p[0], p1 = p[1];
-    a = __builtin_bit_cast(float, p0);
-    b = __builtin_bit_cast(float, p1);
-}
-__device__ __forceinline__ float quad_max(float x) {
-    float a, b;
-    swap_pair(x, false, a, b);
-    swap_pair(fmaxf(a, b), true, a, b);
-    return fmaxf(a, b);
-}
-__device__ __forceinline__ float quad_sum(float x) {
-    float a, b;
-    swap_pair(x, false, a, b);
-    swap_pair(a + b, true, a, b);
-    return a + b;
-}
-
-template <int DT> __device__ __forceinline__ void store_elem(void *base, int64_t i, float x) {
-    if constexpr (DT == F32) reinterpret_cast<float *>(base)[i] = x;
-    else if constexpr (DT == F16) reinterpret_cast<_Float16 *>(base)[i] = (_Float16)x;
-    else reinterpret_cast<__bf16 *>(base)[i] = (__bf16)x;
-}
-template <int DT> __device__ __forceinline__ void store_elem4(void *base, int64_t i, f32x4 x) {
-    if constexpr (DT == F32) *gstore_ptr<f32x4>(reinterpret_cast<float *>(base) + i) = x;
-    else *gstore_ptr<u32x2>(reinterpret_cast<uint16_t *>(base) + i) = pack4<DT>(x);
-}
-
-// Partials pass between workgroups on different XCDs: these go past the L2, so a
-// store that has been acknowledged (wait_loads<0>) is there for every other
-// workgroup's load.  That orders a partial before its arrival count without an
-// agent-scope release and acquire, which write back and invalidate the XCD's
-// whole L2: with them each workgroup of a streaming launch took 28 us longer (4
-// sessions of 100k..131k keys in 4096 workgroups 512 us, in 2048 399 us).
-__device__ __forceinline__ void shared_store(float *p, float x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ float shared_load(const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-
-constexpr int CPOL_SC1 = 16;  // a buffer load past the L2, as shared_load
-// LDS for that many (maximum, mass) pairs.
-__device__ constexpr int pairs_bytes(int pairs) { return (pairs * 8 + 15) / 16 * 16; }
-
-// How far a score may pass the row's maximum before the maximum moves, in log2.
-constexpr float SLACK = 8.0f;
-
-}  // namespace
 
 // The ring of one wave: NS stages of one 16-key block, K rows then V rows of 2D
 // bytes.  Rows hold their 16-byte pieces permuted (piece c of row r at c ^ turn(r)),
 // so that 16 rows read at one feature fall on 16 different bank groups.
-#ifndef PDW
-#define PDW 4
-#endif
-#ifndef PDN
-#define PDN (D == 64 ? 4 : 2)
-#endif
 template <int D> struct DecodeRing {
-    static constexpr int W = PDW;          // waves per workgroup
-    static constexpr int NS = PDN;          // stages per wave
+    static constexpr int W = D == 256 ? 2 : 4;          // waves per workgroup
+    static constexpr int NS = D == 64 ? 4 : 2;          // stages per wave
     static constexpr int row = 2 * D;
     static constexpr int tile = 16 * row;
     static constexpr int stage = 2 * tile;
@@ -180,7 +63,7 @@ __global__ __launch_bounds__(64 * DecodeRing<D>::W) void paged_decode(PagedAtten
         return;
     }
     const int nrows = uniform(sq.n * G), pos0 = uniform(sq.len - sq.n), len = uniform(sq.len);
-    if (nrows == 0) return;
+    if (nrows == 0 || nrows > p.decode_rows) return;
 
     // The blocks that some row sees, and this split's share of them.
     const int first_key = pos0 - p.window + 1 > 0 ? pos0 - p.window + 1 : 0;
@@ -241,8 +124,8 @@ __global__ __launch_bounds__(64 * DecodeRing<D>::W) void paged_decode(PagedAtten
         const int page_next = t + NS < mine ? page_of(t + NS) : 0;
         // Loads of later stages may stay under way.
         const int ahead = mine - 1 - t < NS - 1 ? mine - 1 - t : NS - 1;
-        if (NS >= 4 && ahead >= 3) wait_loads<3 * 2 * L::loads>();
-        else if (NS >= 3 && ahead == 2) wait_loads<2 * 2 * L::loads>();
+        if (NS == 4 && ahead >= 3) wait_loads<3 * 2 * L::loads>();
+        else if (NS == 4 && ahead == 2) wait_loads<2 * 2 * L::loads>();
         else if (ahead >= 1) wait_loads<2 * L::loads>();
         else wait_loads<0>();
         lds_ptr<uint8_t> kt = lds + (wave * L::wave_bytes + (t % NS) * L::stage), vt = kt + L::tile;
