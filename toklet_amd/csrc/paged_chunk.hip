@@ -51,17 +51,33 @@ constexpr float BASE_NONE = -0x1p100f;
 
 }  // namespace
 
-// The ring: NS tiles of 32 keys, K rows then V rows.  Rows hold their 16-byte
-// pieces permuted by the row, so that rows read at one feature spread over the banks.
+// The rings: NS tiles of 32 keys of K, and as many of V, whose tiles are read two
+// iterations after K's.  A tile is runs of 1 KiB, each RR whole rows as one direct
+// load of a wave leaves them, with a few bytes between runs; a row's 16-byte pieces
+// are permuted by its place in the run (piece c at c ^ turn).  The two together
+// spread over all banks both the 16 rows that a K read takes at one feature and the
+// four rows x 64 bytes that a transposing V read takes; and since the permutation
+// touches two bits of c only, a read's address is (x ^ constant) + base + constant.
 template <int D> struct ChunkRing {
     static constexpr int KT = 32, NS = 4;
     static constexpr int row = 2 * D;
-    static constexpr int tile = KT * row;
-    static constexpr int stage = 2 * tile;
-    static constexpr int bytes = NS * stage;
-    static constexpr int runs = tile / 4096;  // 1 KiB runs of a tile per wave
-    __device__ static constexpr int turn(int r) { return D >= 128 ? (5 * r) & 15 : (2 * r + (r >> 2)) & 7; }
-    __device__ static constexpr int at(int r, int c) { return r * row + ((c ^ turn(r)) << 4); }
+    static constexpr int RR = 1024 / row;
+    static constexpr int runs = KT / RR, wave_runs = runs / 4;
+    static constexpr int k_run = 1024 + 16, v_run = D == 256 ? 1024 + 64 : 1024 + 16;
+    static constexpr int k_tile = runs * k_run, v_tile = runs * v_run;
+    static constexpr int v_base = NS * k_tile;
+    static constexpr int bytes = v_base + NS * v_tile;
+    __device__ static constexpr int turn(int rr) {
+        return D == 64 ? ((rr >> 1) & 1) << 2 | ((rr >> 2) & 1) << 1 : (D == 128 ? rr << 2 : rr << 3);
+    }
+    __device__ static constexpr int at(int r, int c, int run) { return r / RR * run + r % RR * row + ((c ^ turn(r % RR)) << 4); }
+    // The bits of a piece that the permutation touches, as those of K's step i (pieces
+    // 2i, 2i + 1) and V's feature block f (pieces 4f .. 4f + 3), and the other bits.
+    static constexpr int bits = D == 64 ? 6 : (D == 128 ? 12 : 8);
+    static constexpr int k_turned(int i) { return (2 * i & bits) << 4; }
+    static constexpr int k_plain(int i) { return (2 * i & ~bits) << 4; }
+    static constexpr int v_turned(int f) { return (4 * f & bits) << 4; }
+    static constexpr int v_plain(int f) { return (4 * f & ~bits) << 4; }
 };
 
 // The tiles of row block `rb` that one of its rows sees, and how many splits share them.
@@ -82,7 +98,7 @@ template <int ROWS> __device__ __forceinline__ ChunkSpan chunk_span(const PagedA
 }
 
 template <int DT, int D, int NB, bool CAP>
-__global__ __launch_bounds__(256, NB == 1 && D <= 128 ? 2 : 1) void paged_chunk(PagedAttend p, int row_blocks) {
+__global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void paged_chunk(PagedAttend p, int row_blocks) {
     using L = ChunkRing<D>;
     constexpr int KT = L::KT, NS = L::NS, ROWS = 128 * NB, QS = D / 16, FB = D / 32;
     __shared__ __attribute__((aligned(1024))) uint8_t lds_mem[L::bytes];
@@ -118,19 +134,18 @@ __global__ __launch_bounds__(256, NB == 1 && D <= 128 ? 2 : 1) void paged_chunk(
     const int t_hi = t_lo + per < span.t_end ? t_lo + per : span.t_end;
     const int tiles = uniform(t_hi > t_lo ? t_hi - t_lo : 0);
 
-    // Direct loads: run i of this wave covers rows 16-byte pieces of 1 KiB.
+    // Direct loads: this wave's runs of a tile, consecutive rows of one page.
     const_ptr<int32_t> table = (const_ptr<int32_t>)(p.b.table + (int64_t)sq.slot * p.b.table_stride);
     const uint8_t *kb = reinterpret_cast<const uint8_t *>(p.k) + (int64_t)kvh * p.l.head_stride * 2;
     const uint8_t *vb = reinterpret_cast<const uint8_t *>(p.v) + (int64_t)kvh * p.l.head_stride * 2;
     const int row_bytes = (int)p.l.row_stride * 2;
-    constexpr int RUN_ROWS = 1024 / L::row;             // rows of one run
-    constexpr int WAVE_ROWS = RUN_ROWS * L::runs;        // 8: rows of this wave's share of a tile
-    uint32_t off[L::runs];
-    for (int i = 0; i < L::runs; ++i) {
-        const int r = wave * WAVE_ROWS + i * RUN_ROWS + lane * 16 / L::row, c = (lane * 16 % L::row) >> 4;
-        off[i] = (uint32_t)((r - wave * WAVE_ROWS) * row_bytes + ((c ^ L::turn(r)) << 4));
+    constexpr int WAVE_ROWS = L::wave_runs * L::RR;  // 8
+    uint32_t off[L::wave_runs];
+    for (int i = 0; i < L::wave_runs; ++i) {
+        const int rr = lane * 16 / L::row, c = (lane * 16 % L::row) >> 4;
+        off[i] = (uint32_t)((i * L::RR + rr) * row_bytes + ((c ^ L::turn(rr)) << 4));
     }
-    const uint32_t lds0 = (uint32_t)uniform((int)(uintptr_t)lds) + (uint32_t)wave * (L::runs * 1024);
+    const uint32_t lds0 = (uint32_t)uniform((int)(uintptr_t)lds);
     bool bad_page = false;
     const int last_entry = (len > 0 ? len - 1 : 0) >> p.l.page_shift;
     // This wave's first key of tile t; keys behind the last one repeat its page.
@@ -139,39 +154,45 @@ __global__ __launch_bounds__(256, NB == 1 && D <= 128 ? 2 : 1) void paged_chunk(
         const int e = key_of(t) >> p.l.page_shift;
         return table[e < last_entry ? e : last_entry];
     };
-    auto issue = [&](int t, int page) {
+    auto issue = [&](auto value, int t, int page) {
+        constexpr bool V = decltype(value)::value;
+        constexpr int RUN = V ? L::v_run : L::k_run, TILE = V ? L::v_tile : L::k_tile;
         if ((uint32_t)page >= (uint32_t)p.l.pages) {
             page = 0;
             bad_page = true;
         }
         const int64_t at = ((int64_t)page * p.l.page_stride + (int64_t)(key_of(t) & ((1 << p.l.page_shift) - 1)) * p.l.row_stride) * 2;
-        const uint8_t *ka = uniform_ptr(kb + at), *va = uniform_ptr(vb + at);
-        const uint32_t m = lds0 + (uint32_t)(t % NS) * L::stage;
-        for (int i = 0; i < L::runs; ++i) lds_load16(ka, off[i], m + i * 1024);
-        for (int i = 0; i < L::runs; ++i) lds_load16(va, off[i], m + L::tile + i * 1024);
+        const uint8_t *a = uniform_ptr((V ? vb : kb) + at);
+        const uint32_t m = lds0 + (V ? L::v_base : 0) + (uint32_t)(t & (NS - 1)) * TILE + (uint32_t)wave * (L::wave_runs * RUN);
+        for (int i = 0; i < L::wave_runs; ++i) lds_load16(a, off[i], m + i * RUN);
     };
+    using K = std::false_type;
+    using V = std::true_type;
+    // Iteration t reads K of tile t + 1 and V of tile t - 1 (one block per wave) or t
+    // (two); it starts the loads of K of tile t + 4 and V of tile t + VA, which
+    // iteration t + 3 reads.  The first ones here, in that order: iterations -4 .. -1.
+    constexpr int VA = NB == 2 ? 3 : 2;
     {
-        int pages[NS - 1];
-        for (int t = 0; t < NS - 1; ++t) pages[t] = t < tiles ? page_of(t) : 0;
-        for (int t = 0; t < NS - 1; ++t)
-            if (t < tiles) issue(t, pages[t]);
+        int pages[NS];
+        for (int t = 0; t < NS; ++t) pages[t] = t < tiles ? page_of(t) : 0;
+        for (int t = 0; t < NS; ++t) {
+            if (t < tiles) issue(K{}, t, pages[t]);
+            const int tv = t - 4 + VA;
+            if (tv >= 0 && tv < tiles) issue(V{}, tv, pages[tv]);
+        }
     }
 
     // This wave's rows: lane row n of block nb.
     const int wave_row = rb * ROWS + wave * 32 * NB;
     const bool works = wave_row < nrows;  // uniform
     u32x4 q[NB][QS];
-    int pos[NB], tok[NB], head[NB];
-    bool real[NB];
+    int pos[NB];  // -2^30 - 1: a row past the last, which sees nothing
     for (int b = 0; b < NB; ++b) {
-        const int r = wave_row + 32 * b + n;
-        real[b] = r < nrows;
-        const int rr = real[b] ? r : nrows - 1;
-        tok[b] = rr / G;
-        head[b] = kvh * G + rr % G;
-        pos[b] = pos0 + tok[b];
+        const int r = wave_row + 32 * b + n, rr = r < nrows ? r : nrows - 1;
+        const int tok = rr / G, head = kvh * G + rr % G;
+        pos[b] = r < nrows ? pos0 + tok : -(1 << 30) - 1;
         for (int s = 0; s < QS; ++s)
-            q[b][s] = *gload_ptr<u32x4>(reinterpret_cast<const uint16_t *>(p.q) + ((int64_t)(sq.q0 + tok[b]) * p.hq + head[b]) * D + 16 * s + 8 * h);
+            q[b][s] = *gload_ptr<u32x4>(reinterpret_cast<const uint16_t *>(p.q) + ((int64_t)(sq.q0 + tok) * p.hq + head) * D + 16 * s + 8 * h);
     }
     const int wave_last = wave_row + 32 * NB - 1 < nrows ? wave_row + 32 * NB - 1 : nrows - 1;
     // Keys that every row of the wave sees: [full_lo, full_hi).
@@ -186,125 +207,214 @@ __global__ __launch_bounds__(256, NB == 1 && D <= 128 ? 2 : 1) void paged_chunk(
     }
     bool bad = false;
 
-    // Scores of tile t for every block.
-    auto scores = [&](int t, f32x16 (&s)[NB]) {
-        lds_ptr<uint8_t> kt = lds + (t % NS) * L::stage;
-        for (int b = 0; b < NB; ++b) s[b] = f32x16{};
-        for (int i = 0; i < QS; ++i) {
-            const u32x4 k = *(lds_ptr<u32x4>)(kt + L::at(n, 2 * i + h));
-            for (int b = 0; b < NB; ++b) s[b] = mfma_32x32x16<DT>(k, q[b][i], s[b]);
-        }
-    };
     auto in_log2 = [&](float s) { return CAP ? tanh_fast(s * p.softcap_y) * p.softcap_log2 : s * p.scale_log2; };
-    // Weights of tile t from its scores, the rows' masses and bases.
-    auto softmax = [&](int t, f32x16 (&s)[NB], u32x4 (&w)[NB][2]) {
+    // A score's weight against a base; a hidden key's score is -inf.
+    auto weight = [&](float s, float from) {
+        float x;
+        if constexpr (CAP) x = s == NEG_INF ? NEG_INF : in_log2(s) - from;
+        else x = __builtin_fmaf(s, p.scale_log2, -from);
+        return __builtin_amdgcn_exp2f(x);
+    };
+    // LDS addresses of this lane's operands: a base and the row's permutation.
+    uint32_t k_base, k_turn, v_base, v_turn;
+    {
+        const int j = lane & 15, r = 4 * h + (j >> 2), c = 2 * ((lane >> 4) & 1) + ((j & 3) >> 1), x = L::turn(r % L::RR);
+        k_turn = (uint32_t)L::turn(n % L::RR) << 4;
+        k_base = lds0 + n / L::RR * L::k_run + n % L::RR * L::row + h * 16;
+        v_turn = (uint32_t)(x & ~3) << 4;
+        v_base = lds0 + L::v_base + r / L::RR * L::v_run + r % L::RR * L::row + ((c ^ (x & 3)) << 4) + (j & 1) * 8;
+    }
+    auto k_operand = [&](uint32_t base, uint32_t turn, int i) { return *(lds_ptr<u32x4>)(uintptr_t)((turn ^ L::k_turned(i)) + base + L::k_plain(i)); };
+    // V^T operand i: feature block i % FB, keys 16 (i / FB) .. + 15.
+    auto v_operand = [&](uint32_t base, uint32_t turn, int i) {
+        const int f = i % FB, first = 16 * (i / FB) / L::RR * L::v_run + L::v_plain(f);
+        const uint32_t x = (turn ^ L::v_turned(f)) + base;
+        const u32x2 a = read_tr((lds_ptr<uint8_t>)(uintptr_t)(x + first)), b = read_tr((lds_ptr<uint8_t>)(uintptr_t)(x + first + 8 / L::RR * L::v_run));
+        return u32x4{a[0], a[1], b[0], b[1]};
+    };
+    auto meet = [&]() {
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    // Until every wave's loads up to iteration t - 3 have arrived and every wave has
+    // left iteration t - 1, whose tiles the next loads overwrite.  What iterations
+    // t - 2 and t - 1 have started may be under way.
+    auto arrive = [&](int t) {
+        const int left = tiles - t;
+        if (left >= 4) wait_loads<4 * L::wave_runs>();
+        else if (left == 3) wait_loads<3 * L::wave_runs>();
+        else if (NB == 1 && left == 2) wait_loads<2 * L::wave_runs>();
+        else if (left == NB) wait_loads<L::wave_runs>();
+        else wait_loads<0>();
+        meet();
+    };
+    // Keys of tile t that no row of the sequence sees are whatever the page holds there,
+    // NaN too: their V rows become zeros before any wave reads them.
+    auto clear_dead = [&](int t) {
         const int key0 = (t_lo + t) << 5;
-        const bool full = key0 >= full_lo && key0 + KT <= full_hi;
-        if (!full) {
-            for (int b = 0; b < NB; ++b)
-                for (int i = 0; i < 16; ++i) {
-                    const int key = key0 + 8 * (i >> 2) + 4 * h + (i & 3);
-                    const bool seen = real[b] && key <= pos[b] && key > pos[b] - p.window;
-                    bad |= seen && !is_finite_f(s[b][i]);
-                    s[b][i] = seen ? s[b][i] : NEG_INF;
-                }
+        if (t < 0 || (key0 >= first_key && key0 + KT <= len)) return;
+        lds_ptr<uint8_t> vt = lds + L::v_base + (t & (NS - 1)) * L::v_tile;
+        for (int i = threadIdx.x; i < KT * L::row / 16; i += 256) {
+            const int r = i * 16 / L::row, key = key0 + r;
+            if (key < first_key || key >= len) *(lds_ptr<u32x4>)(vt + L::at(r, i % (L::row / 16), L::v_run)) = u32x4{};
         }
-        for (int b = 0; b < NB; ++b) {
-            float x[16];
-            float top = 0.0f;
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, __builtin_fabsf(s[b][i]));
-            bad |= full && !(top < __builtin_inff());
-            auto weights = [&]() {
-                float mass = 0.0f;
-                for (int i = 0; i < 16; ++i) {
-                    if constexpr (CAP) x[i] = (full || s[b][i] != NEG_INF) ? in_log2(s[b][i]) - base[b] : NEG_INF;
-                    else x[i] = __builtin_fmaf(s[b][i], p.scale_log2, -base[b]);
-                    x[i] = __builtin_amdgcn_exp2f(x[i]);
-                }
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t v = pack2<DT>(x[2 * j], x[2 * j + 1]);
-                    w[b][j >> 2][j & 3] = v;
-                    mass = add_pair<DT>(v, mass);
-                }
-                return mass;
-            };
-            float mass = weights();
-            if (__ballot(!(mass <= MASS_LIMIT)) != 0) {
-                float mx = NEG_INF;
-                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, (CAP && s[b][i] == NEG_INF) ? NEG_INF : in_log2(s[b][i]));
-                float a0, a1;
-                swap_pair(mx, true, a0, a1);
-                mx = fmaxf(a0, a1);
-                const float next = fmaxf(base[b], mx);
-                const float c = __builtin_amdgcn_exp2f(base[b] - next);
-                base[b] = next;
-                l[b] *= c;
-                for (int f = 0; f < FB; ++f) o[b][f] *= c;
-                mass = weights();
-                bad |= !is_finite_f(mass);
-            }
-            l[b] += mass;
+        wait_lds();
+        meet();
+    };
+    // Whether every row of the wave sees every key of tile t.
+    auto is_full = [&](int t) {
+        const int key0 = (t_lo + t) << 5;
+        return key0 >= full_lo && key0 + KT <= full_hi;
+    };
+    auto hide = [&](int t, int b, f32x16 &s) {
+        const int key0 = ((t_lo + t) << 5) + 4 * h;
+        for (int i = 0; i < 16; ++i) {
+            const int key = key0 + 8 * (i >> 2) + (i & 3);
+            const bool seen = key <= pos[b] && key > pos[b] - p.window;
+            bad |= seen && !is_finite_f(s[i]);
+            s[i] = seen ? s[i] : NEG_INF;
         }
     };
-    // O^T += V^T P^T of tile t.
-    auto values = [&](int t, const u32x4 (&w)[NB][2]) {
-        lds_ptr<uint8_t> vt = lds + (t % NS) * L::stage + L::tile;
-        const int key0 = (t_lo + t) << 5, g = (lane >> 4) & 1, j = lane & 15;
-        const bool dead = key0 < first_key || key0 + KT > len;
-        for (int f = 0; f < FB; ++f)
-            for (int s = 0; s < 2; ++s) {
-                u32x2 v[2];
-                for (int e = 0; e < 2; ++e) {
-                    const int r = 16 * s + 8 * e + 4 * h + (j >> 2);
-                    v[e] = read_tr(vt + L::at(r, 4 * f + 2 * g + ((j & 3) >> 1)) + (j & 1) * 8);
-                    if (dead) {  // whatever the page holds there, NaN too
-                        for (int i = 0; i < 2; ++i) {
-                            const int key = key0 + 16 * s + 8 * e + 4 * h + 2 * i;
-                            v[e][i] &= (key >= first_key && key < len ? 0xffffu : 0u) | (key + 1 >= first_key && key + 1 < len ? 0xffff0000u : 0u);
-                        }
-                    }
-                }
-                const u32x4 a = {v[0][0], v[0][1], v[1][0], v[1][1]};
-                for (int b = 0; b < NB; ++b) o[b][f] = mfma_32x32x16<DT>(a, w[b][s], o[b][f]);
+    // A row's base moves up to the tile's maximum, and the tile's weights are formed again.
+    auto move_base = [&](int b, const f32x16 &s, u32x4 (&w)[2]) {
+        float mx = NEG_INF;
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, (CAP && s[i] == NEG_INF) ? NEG_INF : in_log2(s[i]));
+        float a0, a1;
+        swap_pair(mx, true, a0, a1);
+        const float above = fmaxf(base[b], fmaxf(a0, a1)), c = __builtin_amdgcn_exp2f(base[b] - above);
+        base[b] = above;
+        l[b] *= c;
+        for (int f = 0; f < FB; ++f) o[b][f] *= c;
+        float mass = 0.0f;
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t both = pack2<DT>(weight(s[2 * j], above), weight(s[2 * j + 1], above));
+            w[j >> 2][j & 3] = both;
+            mass = add_pair<DT>(both, mass);
+        }
+        bad |= !is_finite_f(mass);
+        return mass;
+    };
+    // One phase, in eight slots of QS / 4 matrix instructions and the weights of one
+    // pair of keys, which the scheduler keeps in this order: the vector instructions
+    // fill the matrix instructions' time.  It weighs block b's scores `s` of tile t
+    // into w, while values(i) and scores(i) issue the i-th matrix instruction of
+    // another block's or tile's O and S.
+    auto phase = [&](int t, int b, const f32x16 &s, u32x4 (&w)[2], auto values, auto scores) {
+        float mass = 0.0f, top = 0.0f, x0 = 0.0f, x1 = 0.0f;
+        constexpr int OPS = QS / 4;
+        auto pack = [&](int j) {  // the pair that the slot before weighed
+            const uint32_t both = pack2<DT>(x0, x1);
+            w[j >> 2][j & 3] = both;
+            mass = add_pair<DT>(both, mass);
+        };
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int z = 0; z < OPS; ++z) {
+                const int m = u * OPS + z;
+                if (m % 2 == 0) values(m / 2);
+                else scores(m / 2);
             }
+            if (u > 0) pack(u - 1);
+            top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, __builtin_fabsf(s[2 * u])), __builtin_fabsf(s[2 * u + 1]));
+            x0 = weight(s[2 * u], base[b]);
+            x1 = weight(s[2 * u + 1], base[b]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        pack(7);
+        bad |= is_full(t) && !(top < __builtin_inff());
+        if (__builtin_expect(__ballot(!(mass <= MASS_LIMIT)) != 0, 0)) mass = move_base(b, s, w);
+        l[b] += mass;
     };
 
-    // Tile t + 1 has arrived (this wave's loads of tile t + 2 may be under way), and
-    // no wave still reads tile t - 1, whose place tile t + 3 takes.
-    auto next_tile = [&](int t) {
-        const int page = t + NS - 1 < tiles ? page_of(t + NS - 1) : 0;
-        if (t + 2 < tiles) wait_loads<2 * L::runs>();
-        else wait_loads<0>();
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (t + NS - 1 < tiles) issue(t + NS - 1, page);
-    };
-    f32x16 sa[NB], sb[NB];
-    u32x4 w[NB][2];
     if (tiles > 0) {
-        // Tile 0 before the loop.
-        if (tiles > 2) wait_loads<4 * L::runs>();
-        else if (tiles > 1) wait_loads<2 * L::runs>();
-        else wait_loads<0>();
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (works) scores(0, sa);
-        for (int t = 0; t < tiles; t += 2) {
-            next_tile(t);
-            if (works) {
-                if (t + 1 < tiles) scores(t + 1, sb);
-                softmax(t, sa, w);
-                values(t, w);
-            }
+        f32x16 sa, sb;
+        u32x4 wa[2] = {}, wb[2] = {};
+        if constexpr (NB == 2) {
+            // Blocks a and b half an iteration apart: while a's tile t is weighed, b's
+            // values of tile t - 1 and scores of tile t are formed, then the other way
+            // round.  K and V operands stay in registers for both.
+            u32x4 k[QS], v[QS] = {};
+            arrive(0);
+            for (int i = 0; i < QS; ++i) k[i] = k_operand(k_base, k_turn, i);
+            for (int i = 0; i < QS; ++i) sa = mfma_32x32x16<DT>(k[i], q[0][i], i == 0 ? f32x16{} : sa);
             wait_lds();
-            if (t + 1 >= tiles) break;
-            next_tile(t + 1);
-            if (works) {
-                if (t + 2 < tiles) scores(t + 2, sa);
-                softmax(t + 1, sb, w);
-                values(t + 1, w);
+            for (int t = 0; t < tiles; ++t) {
+                const int page_k = t + 4 < tiles ? page_of(t + 4) : 0, page_v = t + VA < tiles ? page_of(t + VA) : 0;
+                arrive(t);
+                if (t + 4 < tiles) issue(K{}, t + 4, page_k);
+                if (t + VA < tiles) issue(V{}, t + VA, page_v);
+                clear_dead(t);
+                if (works) {
+                    const uint32_t ka = k_base + (uint32_t)((t + 1) & (NS - 1)) * L::k_tile, va = v_base + (uint32_t)(t & (NS - 1)) * L::v_tile;
+                    const bool full = is_full(t);
+                    if (!full) hide(t, 0, sa);
+                    phase(t, 0, sa, wa,
+                          [&](int i) {
+                              o[1][i % FB] = mfma_32x32x16<DT>(v[i], wb[i / FB], o[1][i % FB]);
+                              v[i] = v_operand(va, v_turn, i);
+                          },
+                          [&](int i) {
+                              sb = mfma_32x32x16<DT>(k[i], q[1][i], i == 0 ? f32x16{} : sb);
+                              k[i] = k_operand(ka, k_turn, i);
+                          });
+                    if (!full) hide(t, 1, sb);
+                    phase(t, 1, sb, wb, [&](int i) { o[0][i % FB] = mfma_32x32x16<DT>(v[i], wa[i / FB], o[0][i % FB]); },
+                          [&](int i) { sa = mfma_32x32x16<DT>(k[i], q[0][i], i == 0 ? f32x16{} : sa); });
+                }
+                wait_lds();
             }
+            if (works)
+                for (int i = 0; i < QS; ++i) o[1][i % FB] = mfma_32x32x16<DT>(v[i], wb[i / FB], o[1][i % FB]);
+        } else {
+            // Scores of tile t + 1, weights of tile t and values of tile t - 1 together.  The
+            // first iteration adds values and the last forms scores of a tile that is not
+            // there: weights of zero against a cleared tile, and scores that nobody uses.
+            for (int i = threadIdx.x; i < L::v_tile / 16; i += 256) *(lds_ptr<u32x4>)(lds + L::v_base + (NS - 1) * L::v_tile + i * 16) = u32x4{};
             wait_lds();
+            arrive(0);
+            for (int i = 0; i < QS; ++i) sa = mfma_32x32x16<DT>(k_operand(k_base, k_turn, i), q[0][i], i == 0 ? f32x16{} : sa);
+            wait_lds();
+            auto step = [&](int t, f32x16 &now, f32x16 &next, u32x4 (&w)[2], const u32x4 (&before)[2]) {
+                const int page_k = t + 4 < tiles ? page_of(t + 4) : 0, page_v = t + VA < tiles ? page_of(t + VA) : 0;
+                arrive(t);
+                if (t + 4 < tiles) issue(K{}, t + 4, page_k);
+                if (t + VA < tiles) issue(V{}, t + VA, page_v);
+                clear_dead(t - 1);
+                if (works) {
+                    const uint32_t ka = k_base + (uint32_t)((t + 1) & (NS - 1)) * L::k_tile, va = v_base + (uint32_t)((t - 1) & (NS - 1)) * L::v_tile;
+                    if (!is_full(t)) hide(t, 0, now);
+                    // Not the same from iteration to iteration, as far as the compiler knows: it
+                    // would keep a register for each operand's address.
+                    uint32_t kx = k_turn, vx = v_turn;
+                    asm volatile("" : "+v"(kx), "+v"(vx));
+                    u32x4 k = k_operand(ka, kx, 0), v = v_operand(va, vx, 0);
+                    phase(t, 0, now, w,
+                          [&](int i) {
+                              o[0][i % FB] = mfma_32x32x16<DT>(v, before[i / FB], o[0][i % FB]);
+                              if (i + 1 < QS) v = v_operand(va, vx, i + 1);
+                          },
+                          [&](int i) {
+                              next = mfma_32x32x16<DT>(k, q[0][i], i == 0 ? f32x16{} : next);
+                              if (i + 1 < QS) k = k_operand(ka, kx, i + 1);
+                          });
+                }
+                wait_lds();
+            };
+            for (int t = 0;;) {
+                step(t, sa, sb, wa, wb);
+                if (++t == tiles) break;
+                step(t, sb, sa, wb, wa);
+                if (++t == tiles) break;
+            }
+            arrive(tiles);
+            clear_dead(tiles - 1);
+            if (works) {
+                const uint32_t va = v_base + (uint32_t)((tiles - 1) & (NS - 1)) * L::v_tile;
+                for (int i = 0; i < QS; ++i)
+                    o[0][i % FB] = mfma_32x32x16<DT>(v_operand(va, v_turn, i), tiles & 1 ? wa[i / FB] : wb[i / FB], o[0][i % FB]);
+            }
         }
     }
 
@@ -315,19 +425,21 @@ __global__ __launch_bounds__(256, NB == 1 && D <= 128 ? 2 : 1) void paged_chunk(
             float a0, a1;
             swap_pair(l[b], true, a0, a1);
             const float mass = a0 + a1;
-            const int r = wave * 32 * NB + 32 * b + n;  // row in the block
-            if (!real[b]) continue;
+            int r = wave * 32 * NB + 32 * b + n;  // row in the block
+            asm volatile("" : "+v"(r));  // formed again here: nothing of it lives through the loop
+            if (rb * ROWS + r >= nrows) continue;
+            const int tok = (rb * ROWS + r) / G, head = kvh * G + (rb * ROWS + r) % G;
             if (span.active == 1) {
                 const float inv = 1.0f / mass;
                 for (int f = 0; f < FB; ++f)
                     for (int i = 0; i < 4; ++i) {
                         f32x4 y = {};
-                        if (pos[b] >= 0)
+                        if (pos0 + tok >= 0)
                             for (int j = 0; j < 4; ++j) {
                                 y[j] = o[b][f][4 * i + j] * inv;
                                 bad_out |= !is_finite_f(y[j]);
                             }
-                        store_elem4<DT>(p.out, ((int64_t)(sq.q0 + tok[b]) * p.hq + head[b]) * D + 32 * f + 8 * i + 4 * h, y);
+                        store_elem4<DT>(p.out, ((int64_t)(sq.q0 + tok) * p.hq + head) * D + 32 * f + 8 * i + 4 * h, y);
                     }
             } else {
                 for (int f = 0; f < FB; ++f)
