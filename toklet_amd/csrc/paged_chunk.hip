@@ -106,18 +106,25 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
     const int G = p.group;
 
-    // Workgroups reach the XCDs in turn; each XCD takes a contiguous range of the
-    // (sequence, KV head) units, whose row blocks share K and V in its L2.  Within a
-    // unit the longest row blocks and the shortest alternate.
+    // Workgroups reach the XCDs in turn.  Where there are units (sequence, KV head)
+    // enough, each XCD takes a contiguous range of them, whose row blocks share K and V
+    // in its L2; a few are dealt out one by one, or some XCDs would have more work.  A
+    // unit's longest row blocks come first.
     int unit, rb, split;
     {
-        const uint32_t nb = gridDim.x, b = blockIdx.x, x = b % 8, k = b / 8;
-        const uint32_t per = (nb + 7) / 8, full = nb % 8 == 0 ? 8 : nb % 8;
-        const uint32_t t = x < full ? x * per + k : full * per + (x - full) * (per - 1) + k;
-        split = (int)(t % (uint32_t)p.splits);
-        const uint32_t i = t / (uint32_t)p.splits % (uint32_t)row_blocks;
-        unit = (int)(t / (uint32_t)p.splits / (uint32_t)row_blocks);
-        rb = i % 2 == 0 ? row_blocks - 1 - (int)(i / 2) : (int)(i / 2);
+        const uint32_t nb = gridDim.x, b = blockIdx.x, splits = (uint32_t)p.splits, units = (uint32_t)(p.b.sequences * p.hkv);
+        uint32_t rest;
+        if (units % 8 == 0 || units >= 32) {
+            const uint32_t x = b % 8, k = b / 8, per = (nb + 7) / 8, full = nb % 8 == 0 ? 8 : nb % 8;
+            const uint32_t t = x < full ? x * per + k : full * per + (x - full) * (per - 1) + k;
+            unit = (int)(t / splits / (uint32_t)row_blocks);
+            rest = t % (splits * (uint32_t)row_blocks);
+        } else {
+            unit = (int)(b % units);
+            rest = b / units;
+        }
+        split = (int)(rest % splits);
+        rb = row_blocks - 1 - (int)(rest / splits);
     }
     const int kvh = unit % p.hkv;
     const PagedSeq sq = paged_sequence(p.b, unit / p.hkv);
@@ -140,10 +147,10 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
     const uint8_t *vb = reinterpret_cast<const uint8_t *>(p.v) + (int64_t)kvh * p.l.head_stride * 2;
     const int row_bytes = (int)p.l.row_stride * 2;
     constexpr int WAVE_ROWS = L::wave_runs * L::RR;  // 8
-    uint32_t off[L::wave_runs];
-    for (int i = 0; i < L::wave_runs; ++i) {
+    uint32_t off;
+    {
         const int rr = lane * 16 / L::row, c = (lane * 16 % L::row) >> 4;
-        off[i] = (uint32_t)((i * L::RR + rr) * row_bytes + ((c ^ L::turn(rr)) << 4));
+        off = (uint32_t)(rr * row_bytes + ((c ^ L::turn(rr)) << 4));
     }
     const uint32_t lds0 = (uint32_t)uniform((int)(uintptr_t)lds);
     bool bad_page = false;
@@ -164,7 +171,7 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
         const int64_t at = ((int64_t)page * p.l.page_stride + (int64_t)(key_of(t) & ((1 << p.l.page_shift) - 1)) * p.l.row_stride) * 2;
         const uint8_t *a = uniform_ptr((V ? vb : kb) + at);
         const uint32_t m = lds0 + (V ? L::v_base : 0) + (uint32_t)(t & (NS - 1)) * TILE + (uint32_t)wave * (L::wave_runs * RUN);
-        for (int i = 0; i < L::wave_runs; ++i) lds_load16(a, off[i], m + i * RUN);
+        for (int i = 0; i < L::wave_runs; ++i) lds_load16(a + (int64_t)(i * L::RR) * row_bytes, off, m + i * RUN);
     };
     using K = std::false_type;
     using V = std::true_type;
@@ -172,17 +179,9 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
     // (two); it starts the loads of K of tile t + 4 and V of tile t + VA, which
     // iteration t + 3 reads.  The first ones here, in that order: iterations -4 .. -1.
     constexpr int VA = NB == 2 ? 3 : 2;
-    {
-        int pages[NS];
-        for (int t = 0; t < NS; ++t) pages[t] = t < tiles ? page_of(t) : 0;
-        for (int t = 0; t < NS; ++t) {
-            if (t < tiles) issue(K{}, t, pages[t]);
-            const int tv = t - 4 + VA;
-            if (tv >= 0 && tv < tiles) issue(V{}, tv, pages[tv]);
-        }
-    }
-
-    // This wave's rows: lane row n of block nb.
+    // This wave's rows: lane row n of block nb.  Their loads come first, and are waited
+    // for here: the compiler, which does not count the direct loads, would otherwise
+    // wait for Q inside the loop, and with it for all of them.
     const int wave_row = rb * ROWS + wave * 32 * NB;
     const bool works = wave_row < nrows;  // uniform
     u32x4 q[NB][QS];
@@ -194,6 +193,18 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
         for (int s = 0; s < QS; ++s)
             q[b][s] = *gload_ptr<u32x4>(reinterpret_cast<const uint16_t *>(p.q) + ((int64_t)(sq.q0 + tok) * p.hq + head) * D + 16 * s + 8 * h);
     }
+    {
+        int pages[NS];
+        for (int t = 0; t < NS; ++t) pages[t] = t < tiles ? page_of(t) : 0;
+        for (int b = 0; b < NB; ++b)
+            for (int s = 0; s < QS; ++s) asm volatile("" : "+v"(q[b][s]));
+        for (int t = 0; t < NS; ++t) {
+            if (t < tiles) issue(K{}, t, pages[t]);
+            const int tv = t - 4 + VA;
+            if (tv >= 0 && tv < tiles) issue(V{}, tv, pages[tv]);
+        }
+    }
+
     const int wave_last = wave_row + 32 * NB - 1 < nrows ? wave_row + 32 * NB - 1 : nrows - 1;
     // Keys that every row of the wave sees: [full_lo, full_hi).
     const int full_lo = uniform(pos0 + wave_last / G - p.window + 1), full_hi = uniform(pos0 + wave_row / G + 1);
@@ -276,20 +287,28 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
         }
     };
     // A row's base moves up to the tile's maximum, and the tile's weights are formed again.
+    // (Seldom: kept apart into small pieces, so that it takes few registers.)
     auto move_base = [&](int b, const f32x16 &s, u32x4 (&w)[2]) {
         float mx = NEG_INF;
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, (CAP && s[i] == NEG_INF) ? NEG_INF : in_log2(s[i]));
+        for (int i = 0; i < 16; ++i) {
+            mx = fmaxf(mx, (CAP && s[i] == NEG_INF) ? NEG_INF : in_log2(s[i]));
+            __builtin_amdgcn_sched_barrier(0);
+        }
         float a0, a1;
         swap_pair(mx, true, a0, a1);
         const float above = fmaxf(base[b], fmaxf(a0, a1)), c = __builtin_amdgcn_exp2f(base[b] - above);
         base[b] = above;
         l[b] *= c;
-        for (int f = 0; f < FB; ++f) o[b][f] *= c;
+        for (int f = 0; f < FB; ++f) {
+            o[b][f] *= c;
+            __builtin_amdgcn_sched_barrier(0);
+        }
         float mass = 0.0f;
         for (int j = 0; j < 8; ++j) {
             const uint32_t both = pack2<DT>(weight(s[2 * j], above), weight(s[2 * j + 1], above));
             w[j >> 2][j & 3] = both;
             mass = add_pair<DT>(both, mass);
+            __builtin_amdgcn_sched_barrier(0);
         }
         bad |= !is_finite_f(mass);
         return mass;
@@ -299,8 +318,11 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
     // fill the matrix instructions' time.  It weighs block b's scores `s` of tile t
     // into w, while values(i) and scores(i) issue the i-th matrix instruction of
     // another block's or tile's O and S.
-    auto phase = [&](int t, int b, const f32x16 &s, u32x4 (&w)[2], auto values, auto scores) {
+    auto phase = [&](int t, int b, f32x16 &s, u32x4 (&w)[2], auto values, auto scores) {
         float mass = 0.0f, top = 0.0f, x0 = 0.0f, x1 = 0.0f;
+        asm volatile("" : "+v"(s));  // in vector registers, not among the accumulators
+        if constexpr (D == 256)
+            for (int f = 0; f < FB; ++f) asm volatile("" : "+a"(o[0][f]));  // and O among them
         constexpr int OPS = QS / 4;
         auto pack = [&](int j) {  // the pair that the slot before weighed
             const uint32_t both = pack2<DT>(x0, x1);
@@ -402,18 +424,24 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
                 }
                 wait_lds();
             };
+            auto last_values = [&](const u32x4 (&w)[2]) {
+                arrive(tiles);
+                clear_dead(tiles - 1);
+                if (!works) return;
+                const uint32_t va = v_base + (uint32_t)((tiles - 1) & (NS - 1)) * L::v_tile;
+                for (int i = 0; i < QS; ++i) o[0][i % FB] = mfma_32x32x16<DT>(v_operand(va, v_turn, i), w[i / FB], o[0][i % FB]);
+            };
             for (int t = 0;;) {
                 step(t, sa, sb, wa, wb);
-                if (++t == tiles) break;
+                if (++t == tiles) {
+                    last_values(wa);
+                    break;
+                }
                 step(t, sb, sa, wb, wa);
-                if (++t == tiles) break;
-            }
-            arrive(tiles);
-            clear_dead(tiles - 1);
-            if (works) {
-                const uint32_t va = v_base + (uint32_t)((tiles - 1) & (NS - 1)) * L::v_tile;
-                for (int i = 0; i < QS; ++i)
-                    o[0][i % FB] = mfma_32x32x16<DT>(v_operand(va, v_turn, i), tiles & 1 ? wa[i / FB] : wb[i / FB], o[0][i % FB]);
+                if (++t == tiles) {
+                    last_values(wb);
+                    break;
+                }
             }
         }
     }
