@@ -193,9 +193,14 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
         for (int s = 0; s < QS; ++s)
             q[b][s] = *gload_ptr<u32x4>(reinterpret_cast<const uint16_t *>(p.q) + ((int64_t)(sq.q0 + tok) * p.hq + head) * D + 16 * s + 8 * h);
     }
+    // Page numbers: one tile's is loaded an iteration before its K is, and V, later, takes
+    // it from there.
+    int page_k, page_v[4 - VA];
     {
         int pages[NS];
-        for (int t = 0; t < NS; ++t) pages[t] = t < tiles ? page_of(t) : 0;
+        for (int t = 0; t < NS; ++t) pages[t] = page_of(t);
+        page_k = page_of(NS);
+        for (int i = 0; i < 4 - VA; ++i) page_v[i] = pages[VA + i];
         for (int b = 0; b < NB; ++b)
             for (int s = 0; s < QS; ++s) asm volatile("" : "+v"(q[b][s]));
         for (int t = 0; t < NS; ++t) {
@@ -235,14 +240,22 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
         v_turn = (uint32_t)(x & ~3) << 4;
         v_base = lds0 + L::v_base + r / L::RR * L::v_run + r % L::RR * L::row + ((c ^ (x & 3)) << 4) + (j & 1) * 8;
     }
-    auto k_operand = [&](uint32_t base, uint32_t turn, int i) { return *(lds_ptr<u32x4>)(uintptr_t)((turn ^ L::k_turned(i)) + base + L::k_plain(i)); };
+    // An operand's address; opaque, so that the constants after it stay in the loads.
+    auto turned = [&](uint32_t base, uint32_t turn, int bits) {
+        uint32_t x = (turn ^ (uint32_t)bits) + base;
+        asm("" : "+v"(x));
+        return x;
+    };
+    auto k_read = [&](uint32_t at, int i) { return *(lds_ptr<u32x4>)((lds_ptr<uint8_t>)(uintptr_t)at + L::k_plain(i)); };
     // V^T operand i: feature block i % FB, keys 16 (i / FB) .. + 15.
-    auto v_operand = [&](uint32_t base, uint32_t turn, int i) {
-        const int f = i % FB, first = 16 * (i / FB) / L::RR * L::v_run + L::v_plain(f);
-        const uint32_t x = (turn ^ L::v_turned(f)) + base;
-        const u32x2 a = read_tr((lds_ptr<uint8_t>)(uintptr_t)(x + first)), b = read_tr((lds_ptr<uint8_t>)(uintptr_t)(x + first + 8 / L::RR * L::v_run));
+    auto v_read = [&](uint32_t at, int i) {
+        const int first = 16 * (i / FB) / L::RR * L::v_run + L::v_plain(i % FB);
+        lds_ptr<uint8_t> x = (lds_ptr<uint8_t>)(uintptr_t)at;
+        const u32x2 a = read_tr(x + first), b = read_tr(x + first + 8 / L::RR * L::v_run);
         return u32x4{a[0], a[1], b[0], b[1]};
     };
+    auto k_operand = [&](uint32_t base, uint32_t turn, int i) { return k_read(turned(base, turn, L::k_turned(i)), i); };
+    auto v_operand = [&](uint32_t base, uint32_t turn, int i) { return v_read(turned(base, turn, L::v_turned(i % FB)), i); };
     auto meet = [&]() {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -258,6 +271,15 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
         else if (left == NB) wait_loads<L::wave_runs>();
         else wait_loads<0>();
         meet();
+    };
+    // What iteration t starts with: its tiles are there, the next ones' loads begin.
+    auto next_loads = [&](int t) {
+        arrive(t);
+        if (t + 4 < tiles) issue(K{}, t + 4, page_k);
+        if (t + VA < tiles) issue(V{}, t + VA, page_v[0]);
+        if constexpr (VA == 2) page_v[0] = page_v[1];
+        page_v[3 - VA] = page_k;
+        page_k = page_of(t + 5);
     };
     // Keys of tile t that no row of the sequence sees are whatever the page holds there,
     // NaN too: their V rows become zeros before any wave reads them.
@@ -363,10 +385,7 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
             for (int i = 0; i < QS; ++i) sa = mfma_32x32x16<DT>(k[i], q[0][i], i == 0 ? f32x16{} : sa);
             wait_lds();
             for (int t = 0; t < tiles; ++t) {
-                const int page_k = t + 4 < tiles ? page_of(t + 4) : 0, page_v = t + VA < tiles ? page_of(t + VA) : 0;
-                arrive(t);
-                if (t + 4 < tiles) issue(K{}, t + 4, page_k);
-                if (t + VA < tiles) issue(V{}, t + VA, page_v);
+                next_loads(t);
                 clear_dead(t);
                 if (works) {
                     const uint32_t ka = k_base + (uint32_t)((t + 1) & (NS - 1)) * L::k_tile, va = v_base + (uint32_t)(t & (NS - 1)) * L::v_tile;
@@ -399,10 +418,7 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
             for (int i = 0; i < QS; ++i) sa = mfma_32x32x16<DT>(k_operand(k_base, k_turn, i), q[0][i], i == 0 ? f32x16{} : sa);
             wait_lds();
             auto step = [&](int t, f32x16 &now, f32x16 &next, u32x4 (&w)[2], const u32x4 (&before)[2]) {
-                const int page_k = t + 4 < tiles ? page_of(t + 4) : 0, page_v = t + VA < tiles ? page_of(t + VA) : 0;
-                arrive(t);
-                if (t + 4 < tiles) issue(K{}, t + 4, page_k);
-                if (t + VA < tiles) issue(V{}, t + VA, page_v);
+                next_loads(t);
                 clear_dead(t - 1);
                 if (works) {
                     const uint32_t ka = k_base + (uint32_t)((t + 1) & (NS - 1)) * L::k_tile, va = v_base + (uint32_t)((t - 1) & (NS - 1)) * L::v_tile;
