@@ -137,12 +137,12 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
     const ChunkSpan span = chunk_span<ROWS>(p, sq, rb);
     if (split >= span.active) return;
     const int per = (span.t_end - span.t_first + span.active - 1) / span.active;
-    const int t_lo = span.t_first + split * per;
+    const int t_lo = uniform(span.t_first + split * per);
     const int t_hi = t_lo + per < span.t_end ? t_lo + per : span.t_end;
     const int tiles = uniform(t_hi > t_lo ? t_hi - t_lo : 0);
 
     // Direct loads: this wave's runs of a tile, consecutive rows of one page.
-    const_ptr<int32_t> table = (const_ptr<int32_t>)(p.b.table + (int64_t)sq.slot * p.b.table_stride);
+    const_ptr<int32_t> table = (const_ptr<int32_t>)(p.b.table + (int64_t)uniform(sq.slot) * p.b.table_stride);
     const uint8_t *kb = reinterpret_cast<const uint8_t *>(p.k) + (int64_t)kvh * p.l.head_stride * 2;
     const uint8_t *vb = reinterpret_cast<const uint8_t *>(p.v) + (int64_t)kvh * p.l.head_stride * 2;
     const int row_bytes = (int)p.l.row_stride * 2;
@@ -154,24 +154,26 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
     }
     const uint32_t lds0 = (uint32_t)uniform((int)(uintptr_t)lds);
     bool bad_page = false;
-    const int last_entry = (len > 0 ? len - 1 : 0) >> p.l.page_shift;
-    // This wave's first key of tile t; keys behind the last one repeat its page.
-    auto key_of = [&](int t) { return ((t_lo + t) << 5) + wave * WAVE_ROWS; };
+    // This wave's first key of tile t is key_first + 32 t.  A tile's page number is
+    // loaded an iteration before its place is worked out, that one before K's loads, and
+    // V's loads, later, take it from there.  Keys behind the last one repeat its page.
+    const int key_first = (t_lo << 5) + wave * WAVE_ROWS, last_entry = (len > 0 ? len - 1 : 0) >> p.l.page_shift;
+    const uint32_t page_bytes = (uint32_t)p.l.page_stride * 2, page_mask = (1u << p.l.page_shift) - 1;
     auto page_of = [&](int t) {
-        const int e = key_of(t) >> p.l.page_shift;
+        const int e = (key_first + 32 * t) >> p.l.page_shift;
         return table[e < last_entry ? e : last_entry];
     };
-    auto issue = [&](auto value, int t, int page) {
+    auto place_of = [&](int t, int page) {
+        const bool in = (uint32_t)page < (uint32_t)p.l.pages;
+        bad_page |= !in;
+        return (uint64_t)(in ? (uint32_t)page : 0u) * page_bytes + (((uint32_t)(key_first + 32 * t) & page_mask) * (uint32_t)row_bytes);
+    };
+    const uint32_t lds_k = lds0 + (uint32_t)wave * (L::wave_runs * L::k_run), lds_v = lds0 + L::v_base + (uint32_t)wave * (L::wave_runs * L::v_run);
+    auto issue = [&](auto value, int t, uint64_t at) {
         constexpr bool V = decltype(value)::value;
-        constexpr int RUN = V ? L::v_run : L::k_run, TILE = V ? L::v_tile : L::k_tile;
-        if ((uint32_t)page >= (uint32_t)p.l.pages) {
-            page = 0;
-            bad_page = true;
-        }
-        const int64_t at = ((int64_t)page * p.l.page_stride + (int64_t)(key_of(t) & ((1 << p.l.page_shift) - 1)) * p.l.row_stride) * 2;
         const uint8_t *a = uniform_ptr((V ? vb : kb) + at);
-        const uint32_t m = lds0 + (V ? L::v_base : 0) + (uint32_t)(t & (NS - 1)) * TILE + (uint32_t)wave * (L::wave_runs * RUN);
-        for (int i = 0; i < L::wave_runs; ++i) lds_load16(a + (int64_t)(i * L::RR) * row_bytes, off, m + i * RUN);
+        const uint32_t m = V ? lds_v + (uint32_t)(t & (NS - 1)) * L::v_tile : lds_k + (uint32_t)(t & (NS - 1)) * L::k_tile;
+        for (int i = 0; i < L::wave_runs; ++i) lds_load16(a + (uint32_t)(i * L::RR * row_bytes), off, (uint32_t)uniform((int)m) + i * (V ? L::v_run : L::k_run));
     };
     using K = std::false_type;
     using V = std::true_type;
@@ -193,20 +195,22 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
         for (int s = 0; s < QS; ++s)
             q[b][s] = *gload_ptr<u32x4>(reinterpret_cast<const uint16_t *>(p.q) + ((int64_t)(sq.q0 + tok) * p.hq + head) * D + 16 * s + 8 * h);
     }
-    // Page numbers: one tile's is loaded an iteration before its K is, and V, later, takes
-    // it from there.
-    int page_k, page_v[4 - VA];
+    uint64_t at_k, at_v[4 - VA];
+    int page_next;
     {
-        int pages[NS];
-        for (int t = 0; t < NS; ++t) pages[t] = page_of(t);
-        page_k = page_of(NS);
-        for (int i = 0; i < 4 - VA; ++i) page_v[i] = pages[VA + i];
+        int pages[NS + 1];
+        uint64_t at[NS + 1];
+        for (int t = 0; t <= NS; ++t) pages[t] = page_of(t);
+        page_next = page_of(NS + 1);
+        for (int t = 0; t <= NS; ++t) at[t] = place_of(t, pages[t]);
+        at_k = at[NS];
+        for (int i = 0; i < 4 - VA; ++i) at_v[i] = at[VA + i];
         for (int b = 0; b < NB; ++b)
             for (int s = 0; s < QS; ++s) asm volatile("" : "+v"(q[b][s]));
         for (int t = 0; t < NS; ++t) {
-            if (t < tiles) issue(K{}, t, pages[t]);
+            if (t < tiles) issue(K{}, t, at[t]);
             const int tv = t - 4 + VA;
-            if (tv >= 0 && tv < tiles) issue(V{}, tv, pages[tv]);
+            if (tv >= 0 && tv < tiles) issue(V{}, tv, at[tv]);
         }
     }
 
@@ -275,11 +279,12 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
     // What iteration t starts with: its tiles are there, the next ones' loads begin.
     auto next_loads = [&](int t) {
         arrive(t);
-        if (t + 4 < tiles) issue(K{}, t + 4, page_k);
-        if (t + VA < tiles) issue(V{}, t + VA, page_v[0]);
-        if constexpr (VA == 2) page_v[0] = page_v[1];
-        page_v[3 - VA] = page_k;
-        page_k = page_of(t + 5);
+        if (t + 4 < tiles) issue(K{}, t + 4, at_k);
+        if (t + VA < tiles) issue(V{}, t + VA, at_v[0]);
+        if constexpr (VA == 2) at_v[0] = at_v[1];
+        at_v[3 - VA] = at_k;
+        at_k = place_of(t + 5, page_next);
+        page_next = page_of(t + 6);
     };
     // Keys of tile t that no row of the sequence sees are whatever the page holds there,
     // NaN too: their V rows become zeros before any wave reads them.
