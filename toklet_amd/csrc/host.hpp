@@ -151,7 +151,7 @@ struct tkh_context {
     uint32_t *paged_counters = nullptr;  // kPagedCounters arrival counters, 0 between launches, in status_dev's allocation
     int paged_decode_groups = 2048;  // paged decode: workgroups to split towards
     int paged_decode_blocks = 32;    // ... 16-key blocks per split at least
-    int paged_wide_groups = 256;     // paged chunks: 256-row workgroups from which waves take 64 rows
+    int paged_wide_groups = 256;     // paged chunks: 256-row workgroups from which a workgroup has eight waves
     int paged_chunk_groups = 512;    // ... workgroups to split the keys towards
     int paged_chunk_tiles = 8;       // ... 32-key tiles per split at least
     bool test_flag_skew = false; // test hook: merges wait for a flag value no split stores

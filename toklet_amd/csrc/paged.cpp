@@ -13,10 +13,10 @@
 
 extern "C" hipError_t tkh_launch_paged_decode(const tkh::PagedAttend *p, int dtype, int d, hipStream_t stream,
                                               hipEvent_t start, hipEvent_t stop);
-extern "C" int tkh_paged_chunk_blocks(int d);
-extern "C" hipError_t tkh_launch_paged_chunk(const tkh::PagedAttend *p, int dtype, int d, int blocks, int row_blocks,
+extern "C" int tkh_paged_chunk_waves(int d);
+extern "C" hipError_t tkh_launch_paged_chunk(const tkh::PagedAttend *p, int dtype, int d, int waves, int row_blocks,
                                              hipStream_t stream, hipEvent_t start, hipEvent_t stop);
-extern "C" hipError_t tkh_launch_paged_chunk_merge(const tkh::PagedAttend *p, int dtype, int d, int blocks, int row_blocks,
+extern "C" hipError_t tkh_launch_paged_chunk_merge(const tkh::PagedAttend *p, int dtype, int d, int waves, int row_blocks,
                                                    hipStream_t stream, hipEvent_t start, hipEvent_t stop);
 extern "C" hipError_t tkh_launch_paged_rows(const tkh::PagedAttend *p, int dtype, int d, hipStream_t stream,
                                             hipEvent_t start, hipEvent_t stop);
@@ -134,10 +134,10 @@ uint32_t launch_decode(tkh_context *ctx, tkh::PagedAttend p, tkh_dtype dtype, in
 // Sequences of more: the chunk kernel, and where keys are split the merge.
 uint32_t launch_chunk(tkh_context *ctx, tkh::PagedAttend p, tkh_dtype dtype, int D, tkh_error *err) {
     const int64_t rows_each = (int64_t)p.b.max_queries * p.group, units = (int64_t)p.b.sequences * p.hkv;
-    // Two blocks of 32 rows per wave where the row blocks then still fill the CUs.
-    int blocks = tkh_paged_chunk_blocks(D);
-    if (blocks == 2 && p.hkv * ((int64_t)p.b.total * p.group / 256) < ctx->paged_wide_groups) blocks = 1;
-    const int64_t rows = 128 * blocks, row_blocks = (rows_each + rows - 1) / rows;
+    // Eight waves where workgroups of 256 rows still fill the CUs.
+    int waves = tkh_paged_chunk_waves(D);
+    if (waves == 8 && p.hkv * ((int64_t)p.b.total * p.group / 256) < ctx->paged_wide_groups) waves = 4;
+    const int64_t rows = 32 * waves, row_blocks = (rows_each + rows - 1) / rows;
     if (units * row_blocks * 64 > INT32_MAX) return unsupported("paged batch size", err);
     p.rows = (int32_t)rows;
     // The rows that there can be, not what every sequence might have.
@@ -145,10 +145,10 @@ uint32_t launch_chunk(tkh_context *ctx, tkh::PagedAttend p, tkh_dtype dtype, int
     plan_splits(ctx, p, units * row_blocks, ctx->paged_chunk_groups * units * row_blocks / likely, 32, ctx->paged_chunk_tiles, 32, D);
     hipEvent_t *ev = nullptr;
     TRY(profile_events(ctx, p.splits > 1, &ev, err));
-    HIP_TRY(tkh_launch_paged_chunk(&p, (int)dtype, D, blocks, (int)row_blocks, ctx->stream, ev ? ev[0] : nullptr, ev ? ev[1] : nullptr),
+    HIP_TRY(tkh_launch_paged_chunk(&p, (int)dtype, D, waves, (int)row_blocks, ctx->stream, ev ? ev[0] : nullptr, ev ? ev[1] : nullptr),
             "paged chunk launch");
     if (p.splits > 1)
-        HIP_TRY(tkh_launch_paged_chunk_merge(&p, (int)dtype, D, blocks, (int)row_blocks, ctx->stream, ev ? ev[2] : nullptr, ev ? ev[3] : nullptr),
+        HIP_TRY(tkh_launch_paged_chunk_merge(&p, (int)dtype, D, waves, (int)row_blocks, ctx->stream, ev ? ev[2] : nullptr, ev ? ev[3] : nullptr),
                 "paged merge launch");
     return TKH_OK;
 }

@@ -1,8 +1,8 @@
 // paged_chunk.hip - attention of chunks of new tokens over a page table, 16-bit
 // storage: many query rows per KV head, bound by the matrix cores.
 //
-// A workgroup takes 128 NB packed rows (tokens x query heads of one KV head) of one
-// sequence: four waves of NB blocks of 32 rows.  K and V come in tiles of 32 keys
+// A workgroup takes 128 or 256 packed rows (tokens x query heads of one KV head) of one
+// sequence, 32 to a wave.  K and V come in tiles of 32 keys
 // through a ring in LDS, filled by direct global->LDS loads whose page number is
 // uniform in a wave (a load run lies in one 16-key block, and those never leave a
 // page).
@@ -51,22 +51,25 @@ constexpr float BASE_NONE = -0x1p100f;
 
 }  // namespace
 
-// The rings: NS tiles of 32 keys of K, and as many of V, whose tiles are read two
-// iterations after K's.  A tile is runs of 1 KiB, each RR whole rows as one direct
+// The rings: NS groups of TG tiles of 32 keys of K, and as many of V, whose tiles are
+// read two steps after K's.  The waves meet once per group.  A tile is runs of 1 KiB, each RR whole rows as one direct
 // load of a wave leaves them, with a few bytes between runs; a row's 16-byte pieces
 // are permuted by its place in the run (piece c at c ^ turn).  The two together
 // spread over all banks both the 16 rows that a K read takes at one feature and the
 // four rows x 64 bytes that a transposing V read takes; and since the permutation
 // touches two bits of c only, a read's address is (x ^ constant) + base + constant.
-template <int D> struct ChunkRing {
+template <int D, int W> struct ChunkRing {
     static constexpr int KT = 32, NS = 4;
+    static constexpr int TG = W == 8 ? 2 : 1;  // tiles of a group
     static constexpr int row = 2 * D;
     static constexpr int RR = 1024 / row;
-    static constexpr int runs = KT / RR, wave_runs = runs / 4;
+    static constexpr int runs = KT / RR, wave_runs = 8 / RR;  // eight rows of a group per wave
+    static_assert(KT * TG == 8 * W, "a group's rows over its waves");
     static constexpr int k_run = 1024 + 16, v_run = D == 256 ? 1024 + 64 : 1024 + 16;
     static constexpr int k_tile = runs * k_run, v_tile = runs * v_run;
-    static constexpr int v_base = NS * k_tile;
-    static constexpr int bytes = v_base + NS * v_tile;
+    static constexpr int k_group = TG * k_tile, v_group = TG * v_tile;
+    static constexpr int v_base = NS * k_group;
+    static constexpr int bytes = v_base + NS * v_group;
     __device__ static constexpr int turn(int rr) {
         return D == 64 ? ((rr >> 1) & 1) << 2 | ((rr >> 2) & 1) << 1 : (D == 128 ? rr << 2 : rr << 3);
     }
@@ -97,10 +100,10 @@ template <int ROWS> __device__ __forceinline__ ChunkSpan chunk_span(const PagedA
     return s;
 }
 
-template <int DT, int D, int NB, bool CAP>
-__global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void paged_chunk(PagedAttend p, int row_blocks) {
-    using L = ChunkRing<D>;
-    constexpr int KT = L::KT, NS = L::NS, ROWS = 128 * NB, QS = D / 16, FB = D / 32;
+template <int DT, int D, int W, bool CAP>
+__global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chunk(PagedAttend p, int row_blocks) {
+    using L = ChunkRing<D, W>;
+    constexpr int KT = L::KT, NS = L::NS, TG = L::TG, ROWS = 32 * W, QS = D / 16, FB = D / 32;
     __shared__ __attribute__((aligned(1024))) uint8_t lds_mem[L::bytes];
     lds_ptr<uint8_t> lds = (lds_ptr<uint8_t>)lds_mem;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
@@ -141,12 +144,13 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
     const int t_hi = t_lo + per < span.t_end ? t_lo + per : span.t_end;
     const int tiles = uniform(t_hi > t_lo ? t_hi - t_lo : 0);
 
-    // Direct loads: this wave's runs of a tile, consecutive rows of one page.
+    const int groups = (tiles + TG - 1) / TG;
+
+    // Direct loads: this wave's runs of a group, eight rows of one page.
     const_ptr<int32_t> table = (const_ptr<int32_t>)(p.b.table + (int64_t)uniform(sq.slot) * p.b.table_stride);
     const uint8_t *kb = reinterpret_cast<const uint8_t *>(p.k) + (int64_t)kvh * p.l.head_stride * 2;
     const uint8_t *vb = reinterpret_cast<const uint8_t *>(p.v) + (int64_t)kvh * p.l.head_stride * 2;
     const int row_bytes = (int)p.l.row_stride * 2;
-    constexpr int WAVE_ROWS = L::wave_runs * L::RR;  // 8
     uint32_t off;
     {
         const int rr = lane * 16 / L::row, c = (lane * 16 % L::row) >> 4;
@@ -154,77 +158,72 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
     }
     const uint32_t lds0 = (uint32_t)uniform((int)(uintptr_t)lds);
     bool bad_page = false;
-    // This wave's first key of tile t is key_first + 32 t.  A tile's page number is
+    // This wave's first key of group u is key_first + 32 TG u.  A group's page number is
     // loaded an iteration before its place is worked out, that one before K's loads, and
     // V's loads, later, take it from there.  Keys behind the last one repeat its page.
-    const int key_first = (t_lo << 5) + wave * WAVE_ROWS, last_entry = (len > 0 ? len - 1 : 0) >> p.l.page_shift;
+    const int key_first = (t_lo << 5) + wave * 8, last_entry = (len > 0 ? len - 1 : 0) >> p.l.page_shift;
     const uint32_t page_bytes = (uint32_t)p.l.page_stride * 2, page_mask = (1u << p.l.page_shift) - 1;
-    auto page_of = [&](int t) {
-        const int e = (key_first + 32 * t) >> p.l.page_shift;
+    auto page_of = [&](int u) {
+        const int e = (key_first + KT * TG * u) >> p.l.page_shift;
         return table[e < last_entry ? e : last_entry];
     };
-    auto place_of = [&](int t, int page) {
+    auto place_of = [&](int u, int page) {
         const bool in = (uint32_t)page < (uint32_t)p.l.pages;
         bad_page |= !in;
-        return (uint64_t)(in ? (uint32_t)page : 0u) * page_bytes + (((uint32_t)(key_first + 32 * t) & page_mask) * (uint32_t)row_bytes);
+        return (uint64_t)(in ? (uint32_t)page : 0u) * page_bytes + (((uint32_t)(key_first + KT * TG * u) & page_mask) * (uint32_t)row_bytes);
     };
     const uint32_t lds_k = lds0 + (uint32_t)wave * (L::wave_runs * L::k_run), lds_v = lds0 + L::v_base + (uint32_t)wave * (L::wave_runs * L::v_run);
-    auto issue = [&](auto value, int t, uint64_t at) {
+    auto issue = [&](auto value, int u, uint64_t at) {
         constexpr bool V = decltype(value)::value;
         const uint8_t *a = uniform_ptr((V ? vb : kb) + at);
-        const uint32_t m = V ? lds_v + (uint32_t)(t & (NS - 1)) * L::v_tile : lds_k + (uint32_t)(t & (NS - 1)) * L::k_tile;
+        const uint32_t m = V ? lds_v + (uint32_t)(u & (NS - 1)) * L::v_group : lds_k + (uint32_t)(u & (NS - 1)) * L::k_group;
         for (int i = 0; i < L::wave_runs; ++i) lds_load16(a + (uint32_t)(i * L::RR * row_bytes), off, (uint32_t)uniform((int)m) + i * (V ? L::v_run : L::k_run));
     };
     using K = std::false_type;
     using V = std::true_type;
-    // Iteration t reads K of tile t + 1 and V of tile t - 1 (one block per wave) or t
-    // (two); it starts the loads of K of tile t + 4 and V of tile t + VA, which
-    // iteration t + 3 reads.  The first ones here, in that order: iterations -4 .. -1.
-    constexpr int VA = NB == 2 ? 3 : 2;
-    // This wave's rows: lane row n of block nb.  Their loads come first, and are waited
-    // for here: the compiler, which does not count the direct loads, would otherwise
-    // wait for Q inside the loop, and with it for all of them.
-    const int wave_row = rb * ROWS + wave * 32 * NB;
+
+    // This wave's rows: lane row n.  Their loads come first, and are waited for here:
+    // the compiler, which does not count the direct loads, would otherwise wait for Q
+    // inside the loop, and with it for all of them.
+    const int wave_row = rb * ROWS + wave * 32;
     const bool works = wave_row < nrows;  // uniform
-    u32x4 q[NB][QS];
-    int pos[NB];  // -2^30 - 1: a row past the last, which sees nothing
-    for (int b = 0; b < NB; ++b) {
-        const int r = wave_row + 32 * b + n, rr = r < nrows ? r : nrows - 1;
+    u32x4 q[QS];
+    int pos;  // -2^30 - 1: a row past the last, which sees nothing
+    {
+        const int r = wave_row + n, rr = r < nrows ? r : nrows - 1;
         const int tok = rr / G, head = kvh * G + rr % G;
-        pos[b] = r < nrows ? pos0 + tok : -(1 << 30) - 1;
+        pos = r < nrows ? pos0 + tok : -(1 << 30) - 1;
         for (int s = 0; s < QS; ++s)
-            q[b][s] = *gload_ptr<u32x4>(reinterpret_cast<const uint16_t *>(p.q) + ((int64_t)(sq.q0 + tok) * p.hq + head) * D + 16 * s + 8 * h);
+            q[s] = *gload_ptr<u32x4>(reinterpret_cast<const uint16_t *>(p.q) + ((int64_t)(sq.q0 + tok) * p.hq + head) * D + 16 * s + 8 * h);
     }
-    uint64_t at_k, at_v[4 - VA];
+    // Iteration u starts the loads of K of group u + KA and V of group u + VA; the first
+    // ones here, in that order: iterations -KA .. -1.
+    constexpr int KA = TG == 2 ? 3 : 4, VA = 2;
+    uint64_t at_k, at_v[KA - VA];
     int page_next;
     {
-        int pages[NS + 1];
-        uint64_t at[NS + 1];
-        for (int t = 0; t <= NS; ++t) pages[t] = page_of(t);
-        page_next = page_of(NS + 1);
-        for (int t = 0; t <= NS; ++t) at[t] = place_of(t, pages[t]);
-        at_k = at[NS];
-        for (int i = 0; i < 4 - VA; ++i) at_v[i] = at[VA + i];
-        for (int b = 0; b < NB; ++b)
-            for (int s = 0; s < QS; ++s) asm volatile("" : "+v"(q[b][s]));
-        for (int t = 0; t < NS; ++t) {
-            if (t < tiles) issue(K{}, t, at[t]);
-            const int tv = t - 4 + VA;
-            if (tv >= 0 && tv < tiles) issue(V{}, tv, at[tv]);
+        int pages[KA + 1];
+        uint64_t at[KA + 1];
+        for (int u = 0; u <= KA; ++u) pages[u] = page_of(u);
+        page_next = page_of(KA + 1);
+        for (int u = 0; u <= KA; ++u) at[u] = place_of(u, pages[u]);
+        at_k = at[KA];
+        for (int i = 0; i < KA - VA; ++i) at_v[i] = at[VA + i];
+        for (int s = 0; s < QS; ++s) asm volatile("" : "+v"(q[s]));
+        for (int u = 0; u < KA; ++u) {
+            if (u < groups) issue(K{}, u, at[u]);
+            const int uv = u - KA + VA;
+            if (uv >= 0 && uv < groups) issue(V{}, uv, at[uv]);
         }
     }
 
-    const int wave_last = wave_row + 32 * NB - 1 < nrows ? wave_row + 32 * NB - 1 : nrows - 1;
+    const int wave_last = wave_row + 31 < nrows ? wave_row + 31 : nrows - 1;
     // Keys that every row of the wave sees: [full_lo, full_hi).
     const int full_lo = uniform(pos0 + wave_last / G - p.window + 1), full_hi = uniform(pos0 + wave_row / G + 1);
     const int first_key = pos0 - p.window + 1 > 0 ? pos0 - p.window + 1 : 0;
 
-    f32x16 o[NB][FB] = {};
-    float base[NB], l[NB];
-    for (int b = 0; b < NB; ++b) {
-        base[b] = BASE_NONE;
-        l[b] = 0.0f;
-    }
+    f32x16 o[FB] = {};
+    float base = BASE_NONE, l = 0.0f;
     bool bad = false;
 
     auto in_log2 = [&](float s) { return CAP ? tanh_fast(s * p.softcap_y) * p.softcap_log2 : s * p.scale_log2; };
@@ -250,72 +249,87 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
         asm("" : "+v"(x));
         return x;
     };
-    auto k_read = [&](uint32_t at, int i) { return *(lds_ptr<u32x4>)((lds_ptr<uint8_t>)(uintptr_t)at + L::k_plain(i)); };
+    auto k_operand = [&](uint32_t base, uint32_t turn, int i) {
+        return *(lds_ptr<u32x4>)((lds_ptr<uint8_t>)(uintptr_t)turned(base, turn, L::k_turned(i)) + L::k_plain(i));
+    };
     // V^T operand i: feature block i % FB, keys 16 (i / FB) .. + 15.
-    auto v_read = [&](uint32_t at, int i) {
+    auto v_operand = [&](uint32_t base, uint32_t turn, int i) {
         const int first = 16 * (i / FB) / L::RR * L::v_run + L::v_plain(i % FB);
-        lds_ptr<uint8_t> x = (lds_ptr<uint8_t>)(uintptr_t)at;
+        lds_ptr<uint8_t> x = (lds_ptr<uint8_t>)(uintptr_t)turned(base, turn, L::v_turned(i % FB));
         const u32x2 a = read_tr(x + first), b = read_tr(x + first + 8 / L::RR * L::v_run);
         return u32x4{a[0], a[1], b[0], b[1]};
     };
-    auto k_operand = [&](uint32_t base, uint32_t turn, int i) { return k_read(turned(base, turn, L::k_turned(i)), i); };
-    auto v_operand = [&](uint32_t base, uint32_t turn, int i) { return v_read(turned(base, turn, L::v_turned(i % FB)), i); };
+    // Places of a tile in the rings.
+    auto k_place = [&](int t) { return (uint32_t)(t & (NS * TG - 1)) * L::k_tile; };
+    auto v_place = [&](int t) { return (uint32_t)(t & (NS * TG - 1)) * L::v_tile; };
     auto meet = [&]() {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    // Until every wave's loads up to iteration t - 3 have arrived and every wave has
-    // left iteration t - 1, whose tiles the next loads overwrite.  What iterations
-    // t - 2 and t - 1 have started may be under way.
-    auto arrive = [&](int t) {
-        const int left = tiles - t;
-        if (left >= 4) wait_loads<4 * L::wave_runs>();
-        else if (left == 3) wait_loads<3 * L::wave_runs>();
-        else if (NB == 1 && left == 2) wait_loads<2 * L::wave_runs>();
-        else if (left == NB) wait_loads<L::wave_runs>();
-        else wait_loads<0>();
+    // Until the groups that iteration u reads have arrived, and every wave has left
+    // iteration u - 1, whose groups the next loads overwrite.  What the last iteration
+    // (TG 2) or the last two (TG 1) have started may be under way.
+    auto arrive = [&](int u) {
+        const int left = groups - u;
+        if constexpr (TG == 2) {
+            if (left >= 3) wait_loads<2 * L::wave_runs>();
+            else if (left == 2) wait_loads<L::wave_runs>();
+            else wait_loads<0>();
+        } else {
+            if (left >= 4) wait_loads<4 * L::wave_runs>();
+            else if (left == 3) wait_loads<3 * L::wave_runs>();
+            else if (left == 2) wait_loads<2 * L::wave_runs>();
+            else if (left == 1) wait_loads<L::wave_runs>();
+            else wait_loads<0>();
+        }
         meet();
-    };
-    // What iteration t starts with: its tiles are there, the next ones' loads begin.
-    auto next_loads = [&](int t) {
-        arrive(t);
-        if (t + 4 < tiles) issue(K{}, t + 4, at_k);
-        if (t + VA < tiles) issue(V{}, t + VA, at_v[0]);
-        if constexpr (VA == 2) at_v[0] = at_v[1];
-        at_v[3 - VA] = at_k;
-        at_k = place_of(t + 5, page_next);
-        page_next = page_of(t + 6);
     };
     // Keys of tile t that no row of the sequence sees are whatever the page holds there,
     // NaN too: their V rows become zeros before any wave reads them.
     auto clear_dead = [&](int t) {
         const int key0 = (t_lo + t) << 5;
-        if (t < 0 || (key0 >= first_key && key0 + KT <= len)) return;
-        lds_ptr<uint8_t> vt = lds + L::v_base + (t & (NS - 1)) * L::v_tile;
-        for (int i = threadIdx.x; i < KT * L::row / 16; i += 256) {
+        if (t < 0 || t >= tiles || (key0 >= first_key && key0 + KT <= len)) return;
+        lds_ptr<uint8_t> vt = lds + L::v_base + v_place(t);
+        for (int i = threadIdx.x; i < KT * L::row / 16; i += 64 * W) {
             const int r = i * 16 / L::row, key = key0 + r;
             if (key < first_key || key >= len) *(lds_ptr<u32x4>)(vt + L::at(r, i % (L::row / 16), L::v_run)) = u32x4{};
         }
         wait_lds();
         meet();
     };
+    // What iteration u starts with: its tiles are there, the next ones' loads begin.
+    auto next_loads = [&](int u) {
+        arrive(u);
+        if (u + KA < groups) issue(K{}, u + KA, at_k);
+        if (u + VA < groups) issue(V{}, u + VA, at_v[0]);
+        for (int i = 0; i + 1 < KA - VA; ++i) at_v[i] = at_v[i + 1];
+        at_v[KA - VA - 1] = at_k;
+        at_k = place_of(u + KA + 1, page_next);
+        page_next = page_of(u + KA + 2);
+        if constexpr (TG == 2) {
+            clear_dead(2 * u);
+            clear_dead(2 * u + 1);
+        } else {
+            clear_dead(u - 1);
+        }
+    };
     // Whether every row of the wave sees every key of tile t.
     auto is_full = [&](int t) {
         const int key0 = (t_lo + t) << 5;
         return key0 >= full_lo && key0 + KT <= full_hi;
     };
-    auto hide = [&](int t, int b, f32x16 &s) {
+    auto hide = [&](int t, f32x16 &s) {
         const int key0 = ((t_lo + t) << 5) + 4 * h;
         for (int i = 0; i < 16; ++i) {
             const int key = key0 + 8 * (i >> 2) + (i & 3);
-            const bool seen = key <= pos[b] && key > pos[b] - p.window;
+            const bool seen = key <= pos && key > pos - p.window;
             bad |= seen && !is_finite_f(s[i]);
             s[i] = seen ? s[i] : NEG_INF;
         }
     };
     // A row's base moves up to the tile's maximum, and the tile's weights are formed again.
     // (Seldom: kept apart into small pieces, so that it takes few registers.)
-    auto move_base = [&](int b, const f32x16 &s, u32x4 (&w)[2]) {
+    auto move_base = [&](const f32x16 &s, u32x4 (&w)[2]) {
         float mx = NEG_INF;
         for (int i = 0; i < 16; ++i) {
             mx = fmaxf(mx, (CAP && s[i] == NEG_INF) ? NEG_INF : in_log2(s[i]));
@@ -323,11 +337,11 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
         }
         float a0, a1;
         swap_pair(mx, true, a0, a1);
-        const float above = fmaxf(base[b], fmaxf(a0, a1)), c = __builtin_amdgcn_exp2f(base[b] - above);
-        base[b] = above;
-        l[b] *= c;
+        const float above = fmaxf(base, fmaxf(a0, a1)), c = __builtin_amdgcn_exp2f(base - above);
+        base = above;
+        l *= c;
         for (int f = 0; f < FB; ++f) {
-            o[b][f] *= c;
+            o[f] *= c;
             __builtin_amdgcn_sched_barrier(0);
         }
         float mass = 0.0f;
@@ -340,17 +354,25 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
         bad |= !is_finite_f(mass);
         return mass;
     };
-    // One phase, in eight slots of QS / 4 matrix instructions and the weights of one
-    // pair of keys, which the scheduler keeps in this order: the vector instructions
-    // fill the matrix instructions' time.  It weighs block b's scores `s` of tile t
-    // into w, while values(i) and scores(i) issue the i-th matrix instruction of
-    // another block's or tile's O and S.
-    auto phase = [&](int t, int b, f32x16 &s, u32x4 (&w)[2], auto values, auto scores) {
-        float mass = 0.0f, top = 0.0f, x0 = 0.0f, x1 = 0.0f;
-        asm volatile("" : "+v"(s));  // in vector registers, not among the accumulators
+    // Scores of tile t + 1, weights of tile t and values of tile t - 1 together, in eight
+    // slots of QS / 4 matrix instructions and the weights of one pair of keys, which the
+    // scheduler keeps in this order: the vector instructions fill the matrix
+    // instructions' time.  The first step adds values and the last forms scores of a tile
+    // that is not there: weights of zero against a cleared tile, and scores that nobody
+    // uses.
+    auto step = [&](int t, f32x16 &now, f32x16 &next, u32x4 (&w)[2], const u32x4 (&before)[2]) {
+        const uint32_t ka = k_base + k_place(t + 1), va = v_base + v_place(t - 1);
+        const bool full = is_full(t);
+        if (!full) hide(t, now);
+        // Not the same from step to step, as far as the compiler knows: it would keep a
+        // register for each operand's address.
+        uint32_t kx = k_turn, vx = v_turn;
+        asm volatile("" : "+v"(kx), "+v"(vx));
+        asm volatile("" : "+v"(now));  // in vector registers, not among the accumulators
         if constexpr (D == 256)
-            for (int f = 0; f < FB; ++f) asm volatile("" : "+a"(o[0][f]));  // and O among them
-        constexpr int OPS = QS / 4;
+            for (int f = 0; f < FB; ++f) asm volatile("" : "+a"(o[f]));  // and O among them
+        u32x4 k = k_operand(ka, kx, 0), v = v_operand(va, vx, 0);
+        float mass = 0.0f, top = 0.0f, x0 = 0.0f, x1 = 0.0f;
         auto pack = [&](int j) {  // the pair that the slot before weighed
             const uint32_t both = pack2<DT>(x0, x1);
             w[j >> 2][j & 3] = both;
@@ -360,145 +382,95 @@ __global__ __launch_bounds__(256, D == 64 || (NB == 1 && D == 128) ? 2 : 1) void
         for (int u = 0; u < 8; ++u) {
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int z = 0; z < OPS; ++z) {
-                const int m = u * OPS + z;
-                if (m % 2 == 0) values(m / 2);
-                else scores(m / 2);
+            for (int z = 0; z < QS / 4; ++z) {
+                const int m = u * (QS / 4) + z, i = m / 2;
+                if (m % 2 == 0) {
+                    o[i % FB] = mfma_32x32x16<DT>(v, before[i / FB], o[i % FB]);
+                    if (i + 1 < QS) v = v_operand(va, vx, i + 1);
+                } else {
+                    next = mfma_32x32x16<DT>(k, q[i], i == 0 ? f32x16{} : next);
+                    if (i + 1 < QS) k = k_operand(ka, kx, i + 1);
+                }
             }
             if (u > 0) pack(u - 1);
-            top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, __builtin_fabsf(s[2 * u])), __builtin_fabsf(s[2 * u + 1]));
-            x0 = weight(s[2 * u], base[b]);
-            x1 = weight(s[2 * u + 1], base[b]);
+            top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, __builtin_fabsf(now[2 * u])), __builtin_fabsf(now[2 * u + 1]));
+            x0 = weight(now[2 * u], base);
+            x1 = weight(now[2 * u + 1], base);
         }
         __builtin_amdgcn_sched_barrier(0);
         pack(7);
-        bad |= is_full(t) && !(top < __builtin_inff());
-        if (__builtin_expect(__ballot(!(mass <= MASS_LIMIT)) != 0, 0)) mass = move_base(b, s, w);
-        l[b] += mass;
+        bad |= full && !(top < __builtin_inff());
+        if (__builtin_expect(__ballot(!(mass <= MASS_LIMIT)) != 0, 0)) mass = move_base(now, w);
+        l += mass;
     };
 
+    for (int i = threadIdx.x; i < L::v_group / 16; i += 64 * W) *(lds_ptr<u32x4>)(lds + L::v_base + (NS - 1) * L::v_group + i * 16) = u32x4{};
+    wait_lds();
     if (tiles > 0) {
         f32x16 sa, sb;
         u32x4 wa[2] = {}, wb[2] = {};
-        if constexpr (NB == 2) {
-            // Blocks a and b half an iteration apart: while a's tile t is weighed, b's
-            // values of tile t - 1 and scores of tile t are formed, then the other way
-            // round.  K and V operands stay in registers for both.
-            u32x4 k[QS], v[QS] = {};
-            arrive(0);
-            for (int i = 0; i < QS; ++i) k[i] = k_operand(k_base, k_turn, i);
-            for (int i = 0; i < QS; ++i) sa = mfma_32x32x16<DT>(k[i], q[0][i], i == 0 ? f32x16{} : sa);
-            wait_lds();
-            for (int t = 0; t < tiles; ++t) {
-                next_loads(t);
-                clear_dead(t);
-                if (works) {
-                    const uint32_t ka = k_base + (uint32_t)((t + 1) & (NS - 1)) * L::k_tile, va = v_base + (uint32_t)(t & (NS - 1)) * L::v_tile;
-                    const bool full = is_full(t);
-                    if (!full) hide(t, 0, sa);
-                    phase(t, 0, sa, wa,
-                          [&](int i) {
-                              o[1][i % FB] = mfma_32x32x16<DT>(v[i], wb[i / FB], o[1][i % FB]);
-                              v[i] = v_operand(va, v_turn, i);
-                          },
-                          [&](int i) {
-                              sb = mfma_32x32x16<DT>(k[i], q[1][i], i == 0 ? f32x16{} : sb);
-                              k[i] = k_operand(ka, k_turn, i);
-                          });
-                    if (!full) hide(t, 1, sb);
-                    phase(t, 1, sb, wb, [&](int i) { o[0][i % FB] = mfma_32x32x16<DT>(v[i], wa[i / FB], o[0][i % FB]); },
-                          [&](int i) { sa = mfma_32x32x16<DT>(k[i], q[0][i], i == 0 ? f32x16{} : sa); });
-                }
-                wait_lds();
-            }
-            if (works)
-                for (int i = 0; i < QS; ++i) o[1][i % FB] = mfma_32x32x16<DT>(v[i], wb[i / FB], o[1][i % FB]);
-        } else {
-            // Scores of tile t + 1, weights of tile t and values of tile t - 1 together.  The
-            // first iteration adds values and the last forms scores of a tile that is not
-            // there: weights of zero against a cleared tile, and scores that nobody uses.
-            for (int i = threadIdx.x; i < L::v_tile / 16; i += 256) *(lds_ptr<u32x4>)(lds + L::v_base + (NS - 1) * L::v_tile + i * 16) = u32x4{};
-            wait_lds();
-            arrive(0);
-            for (int i = 0; i < QS; ++i) sa = mfma_32x32x16<DT>(k_operand(k_base, k_turn, i), q[0][i], i == 0 ? f32x16{} : sa);
-            wait_lds();
-            auto step = [&](int t, f32x16 &now, f32x16 &next, u32x4 (&w)[2], const u32x4 (&before)[2]) {
-                next_loads(t);
-                clear_dead(t - 1);
-                if (works) {
-                    const uint32_t ka = k_base + (uint32_t)((t + 1) & (NS - 1)) * L::k_tile, va = v_base + (uint32_t)((t - 1) & (NS - 1)) * L::v_tile;
-                    if (!is_full(t)) hide(t, 0, now);
-                    // Not the same from iteration to iteration, as far as the compiler knows: it
-                    // would keep a register for each operand's address.
-                    uint32_t kx = k_turn, vx = v_turn;
-                    asm volatile("" : "+v"(kx), "+v"(vx));
-                    u32x4 k = k_operand(ka, kx, 0), v = v_operand(va, vx, 0);
-                    phase(t, 0, now, w,
-                          [&](int i) {
-                              o[0][i % FB] = mfma_32x32x16<DT>(v, before[i / FB], o[0][i % FB]);
-                              if (i + 1 < QS) v = v_operand(va, vx, i + 1);
-                          },
-                          [&](int i) {
-                              next = mfma_32x32x16<DT>(k, q[0][i], i == 0 ? f32x16{} : next);
-                              if (i + 1 < QS) k = k_operand(ka, kx, i + 1);
-                          });
-                }
-                wait_lds();
-            };
-            auto last_values = [&](const u32x4 (&w)[2]) {
+        arrive(0);
+        for (int i = 0; i < QS; ++i) sa = mfma_32x32x16<DT>(k_operand(k_base, k_turn, i), q[i], i == 0 ? f32x16{} : sa);
+        wait_lds();
+        auto last_values = [&](const u32x4 (&w)[2]) {
+            if constexpr (TG == 1) {
                 arrive(tiles);
                 clear_dead(tiles - 1);
-                if (!works) return;
-                const uint32_t va = v_base + (uint32_t)((tiles - 1) & (NS - 1)) * L::v_tile;
-                for (int i = 0; i < QS; ++i) o[0][i % FB] = mfma_32x32x16<DT>(v_operand(va, v_turn, i), w[i / FB], o[0][i % FB]);
-            };
-            for (int t = 0;;) {
-                step(t, sa, sb, wa, wb);
-                if (++t == tiles) {
-                    last_values(wa);
-                    break;
-                }
-                step(t, sb, sa, wb, wa);
-                if (++t == tiles) {
-                    last_values(wb);
-                    break;
-                }
             }
+            if (!works) return;
+            const uint32_t va = v_base + v_place(tiles - 1);
+            for (int i = 0; i < QS; ++i) o[i % FB] = mfma_32x32x16<DT>(v_operand(va, v_turn, i), w[i / FB], o[i % FB]);
+        };
+        for (int t = 0;;) {
+            next_loads(t / TG);
+            if (works) step(t, sa, sb, wa, wb);
+            if (++t == tiles) {
+                last_values(wa);
+                break;
+            }
+            if constexpr (TG == 1) {
+                wait_lds();
+                next_loads(t);
+            }
+            if (works) step(t, sb, sa, wb, wa);
+            if (++t == tiles) {
+                last_values(wb);
+                break;
+            }
+            wait_lds();
         }
     }
 
     bool bad_out = false;
     const int64_t slot = ((int64_t)unit * row_blocks + rb) * p.splits + split;
-    if (works)
-        for (int b = 0; b < NB; ++b) {
-            float a0, a1;
-            swap_pair(l[b], true, a0, a1);
-            const float mass = a0 + a1;
-            int r = wave * 32 * NB + 32 * b + n;  // row in the block
-            asm volatile("" : "+v"(r));  // formed again here: nothing of it lives through the loop
-            if (rb * ROWS + r >= nrows) continue;
-            const int tok = (rb * ROWS + r) / G, head = kvh * G + (rb * ROWS + r) % G;
-            if (span.active == 1) {
-                const float inv = 1.0f / mass;
-                for (int f = 0; f < FB; ++f)
-                    for (int i = 0; i < 4; ++i) {
-                        f32x4 y = {};
-                        if (pos0 + tok >= 0)
-                            for (int j = 0; j < 4; ++j) {
-                                y[j] = o[b][f][4 * i + j] * inv;
-                                bad_out |= !is_finite_f(y[j]);
-                            }
-                        store_elem4<DT>(p.out, ((int64_t)(sq.q0 + tok) * p.hq + head) * D + 32 * f + 8 * i + 4 * h, y);
-                    }
-            } else {
-                for (int f = 0; f < FB; ++f)
-                    for (int i = 0; i < 4; ++i) {
-                        const f32x4 y = {o[b][f][4 * i], o[b][f][4 * i + 1], o[b][f][4 * i + 2], o[b][f][4 * i + 3]};
-                        *gstore_ptr<f32x4>(p.part_o + (slot * ROWS + r) * D + 32 * f + 8 * i + 4 * h) = y;
-                    }
-                if (h == 0) *gstore_ptr<f32x2>(p.part_ml + (slot * ROWS + r) * 2) = f32x2{base[b], mass};
-            }
+    float a0, a1;
+    swap_pair(l, true, a0, a1);
+    const float mass = a0 + a1;
+    int r = wave * 32 + n;  // row in the block
+    asm volatile("" : "+v"(r));  // formed again here: nothing of it lives through the loop
+    if (rb * ROWS + r < nrows) {
+        const int tok = (rb * ROWS + r) / G, head = kvh * G + (rb * ROWS + r) % G;
+        if (span.active == 1) {
+            const float inv = 1.0f / mass;
+            for (int f = 0; f < FB; ++f)
+                for (int i = 0; i < 4; ++i) {
+                    f32x4 y = {};
+                    if (pos0 + tok >= 0)
+                        for (int j = 0; j < 4; ++j) {
+                            y[j] = o[f][4 * i + j] * inv;
+                            bad_out |= !is_finite_f(y[j]);
+                        }
+                    store_elem4<DT>(p.out, ((int64_t)(sq.q0 + tok) * p.hq + head) * D + 32 * f + 8 * i + 4 * h, y);
+                }
+        } else {
+            for (int f = 0; f < FB; ++f)
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 y = {o[f][4 * i], o[f][4 * i + 1], o[f][4 * i + 2], o[f][4 * i + 3]};
+                    *gstore_ptr<f32x4>(p.part_o + (slot * ROWS + r) * D + 32 * f + 8 * i + 4 * h) = y;
+                }
+            if (h == 0) *gstore_ptr<f32x2>(p.part_ml + (slot * ROWS + r) * 2) = f32x2{base, mass};
         }
+    }
     raise_status(p.status, bad_page, ST_BAD_PAGE);
     raise_status(p.status, bad, ST_NONFINITE_INPUT);
     raise_status(p.status, bad_out, ST_NONFINITE_OUTPUT);
@@ -551,16 +523,16 @@ __global__ __launch_bounds__(256) void paged_chunk_merge(PagedAttend p, int row_
 
 namespace {
 
-template <class F> hipError_t chunk_build(int dtype, int d, int blocks, bool cap, F f) {
+template <class F> hipError_t chunk_build(int dtype, int d, int waves, bool cap, F f) {
     using namespace tkh;
-    auto caps = [&](auto dt, auto dims, auto nb) {
-        return cap ? f(dt, dims, nb, std::true_type{}) : f(dt, dims, nb, std::false_type{});
+    auto caps = [&](auto dt, auto dims, auto w) {
+        return cap ? f(dt, dims, w, std::true_type{}) : f(dt, dims, w, std::false_type{});
     };
     auto rows = [&](auto dt, auto dims) {
         if constexpr (decltype(dims)::value <= 128) {
-            if (blocks == 2) return caps(dt, dims, std::integral_constant<int, 2>{});
+            if (waves == 8) return caps(dt, dims, std::integral_constant<int, 8>{});
         }
-        return caps(dt, dims, std::integral_constant<int, 1>{});
+        return caps(dt, dims, std::integral_constant<int, 4>{});
     };
     auto heads = [&](auto dt) {
         if (d == 64) return rows(dt, std::integral_constant<int, 64>{});
@@ -574,23 +546,24 @@ template <class F> hipError_t chunk_build(int dtype, int d, int blocks, bool cap
 
 }  // namespace
 
-// Blocks of 32 rows a wave of the chunk kernel may take.
-extern "C" int tkh_paged_chunk_blocks(int d) { return d <= 128 ? 2 : 1; }
+// Most waves of a chunk workgroup, 32 rows each (it has these or 4).
+extern "C" int tkh_paged_chunk_waves(int d) { return d <= 128 ? 8 : 4; }
 
-extern "C" hipError_t tkh_launch_paged_chunk(const tkh::PagedAttend *p, int dtype, int d, int blocks, int row_blocks,
+extern "C" hipError_t tkh_launch_paged_chunk(const tkh::PagedAttend *p, int dtype, int d, int waves, int row_blocks,
                                              hipStream_t stream, hipEvent_t start, hipEvent_t stop) {
     const int64_t groups = (int64_t)p->b.sequences * p->hkv * row_blocks * p->splits;
-    return chunk_build(dtype, d, blocks, p->softcap_y != 0.0f, [&](auto dt, auto dims, auto nb, auto cap) {
-        hipExtLaunchKernelGGL((tkh::paged_chunk<decltype(dt)::value, decltype(dims)::value, decltype(nb)::value, decltype(cap)::value>),
-                              dim3((unsigned)groups), dim3(256), 0, stream, start, stop, 0, *p, row_blocks);
+    return chunk_build(dtype, d, waves, p->softcap_y != 0.0f, [&](auto dt, auto dims, auto w, auto cap) {
+        constexpr int W = decltype(w)::value;
+        hipExtLaunchKernelGGL((tkh::paged_chunk<decltype(dt)::value, decltype(dims)::value, W, decltype(cap)::value>),
+                              dim3((unsigned)groups), dim3(64 * W), 0, stream, start, stop, 0, *p, row_blocks);
         return hipGetLastError();
     });
 }
 
-extern "C" hipError_t tkh_launch_paged_chunk_merge(const tkh::PagedAttend *p, int dtype, int d, int blocks, int row_blocks,
+extern "C" hipError_t tkh_launch_paged_chunk_merge(const tkh::PagedAttend *p, int dtype, int d, int waves, int row_blocks,
                                                    hipStream_t stream, hipEvent_t start, hipEvent_t stop) {
-    return chunk_build(dtype, d, blocks, false, [&](auto dt, auto dims, auto nb, auto) {
-        constexpr int D = decltype(dims)::value, ROWS = 128 * decltype(nb)::value, PER = 256 / (D / 4);
+    return chunk_build(dtype, d, waves, false, [&](auto dt, auto dims, auto w, auto) {
+        constexpr int D = decltype(dims)::value, ROWS = 32 * decltype(w)::value, PER = 256 / (D / 4);
         const int64_t groups = (int64_t)p->b.sequences * p->hkv * row_blocks * (ROWS / PER);
         hipExtLaunchKernelGGL((tkh::paged_chunk_merge<decltype(dt)::value, D, ROWS>), dim3((unsigned)groups), dim3(256), 0, stream,
                               start, stop, 0, *p, row_blocks);
