@@ -11,15 +11,13 @@
 #include "host.hpp"
 #include "paged.hpp"
 
-extern "C" hipError_t tkh_launch_paged_decode(const tkh::PagedAttend *p, int dtype, int d, hipStream_t stream,
+extern "C" hipError_t tkh_launch_paged_decode(const tkh::PagedAttend *p, int dtype, int d, int row_blocks, hipStream_t stream,
                                               hipEvent_t start, hipEvent_t stop);
 extern "C" int tkh_paged_chunk_waves(int d);
 extern "C" hipError_t tkh_launch_paged_chunk(const tkh::PagedAttend *p, int dtype, int d, int waves, int row_blocks,
                                              hipStream_t stream, hipEvent_t start, hipEvent_t stop);
 extern "C" hipError_t tkh_launch_paged_chunk_merge(const tkh::PagedAttend *p, int dtype, int d, int waves, int row_blocks,
                                                    hipStream_t stream, hipEvent_t start, hipEvent_t stop);
-extern "C" hipError_t tkh_launch_paged_rows(const tkh::PagedAttend *p, int dtype, int d, hipStream_t stream,
-                                            hipEvent_t start, hipEvent_t stop);
 extern "C" hipError_t tkh_launch_paged_produce(const tkh::PagedProduce *p, int src, int dst, hipStream_t stream);
 extern "C" hipError_t tkh_launch_copy_pages(const tkh::CopyPages *c, hipStream_t stream);
 extern "C" hipError_t tkh_launch_patch_words(const tkh::PatchWords *w, hipStream_t stream);
@@ -119,15 +117,22 @@ void plan_splits(const tkh_context *ctx, tkh::PagedAttend &p, int64_t units, int
     p.counters = ctx->paged_counters;
 }
 
-// Sequences of at most 16 packed rows: paged_decode.
+// paged_decode: sequences of at most 16 packed rows; with FP32 storage, all.
 uint32_t launch_decode(tkh_context *ctx, tkh::PagedAttend p, tkh_dtype dtype, int D, tkh_error *err) {
-    const int64_t units = (int64_t)p.b.sequences * p.hkv;
-    p.rows = (int32_t)std::min<int64_t>((int64_t)p.b.max_queries * p.group, p.decode_rows);
-    plan_splits(ctx, p, units, ctx->paged_decode_groups, 16, ctx->paged_decode_blocks,
+    const int64_t most = std::min<int64_t>((int64_t)p.b.max_queries * p.group, p.decode_rows);
+    // Up to 16 rows a block, so that a batch of single tokens stores partials of its own
+    // rows only; more rows (FP32 storage) in blocks of 32.
+    p.rows = (int32_t)(most <= 16 ? most : 32);
+    const int64_t row_blocks = (most + p.rows - 1) / p.rows, units = (int64_t)p.b.sequences * p.hkv * row_blocks;
+    if (row_blocks > 65535) return unsupported("paged batch size", err);
+    // The rows that there can be, not what every sequence might have.
+    const int64_t likely = std::min<int64_t>(units, p.hkv * (((int64_t)p.b.total * p.group + p.rows - 1) / p.rows + p.b.sequences));
+    plan_splits(ctx, p, units, ctx->paged_decode_groups * units / likely, 16, ctx->paged_decode_blocks,
                 units > kPagedCounters ? 1 : tkh::PAGED_PAIRS_MAX / p.rows, D);
     hipEvent_t *ev = nullptr;
     TRY(profile_events(ctx, false, &ev, err));
-    HIP_TRY(tkh_launch_paged_decode(&p, (int)dtype, D, ctx->stream, ev ? ev[0] : nullptr, ev ? ev[1] : nullptr), "paged decode launch");
+    HIP_TRY(tkh_launch_paged_decode(&p, (int)dtype, D, (int)row_blocks, ctx->stream, ev ? ev[0] : nullptr, ev ? ev[1] : nullptr),
+            "paged decode launch");
     return TKH_OK;
 }
 
@@ -247,16 +252,10 @@ uint32_t tkh_paged_attention(tkh_context *ctx, const tkh_paged_batch *batch, con
     p.status = ctx->status_dev;
     HIP_TRY(hipSetDevice(ctx->device), "hipSetDevice");
     const int D = (int)layout->head_dim;
-    if (dtype == TKH_F32) {
-        hipEvent_t *ev = nullptr;
-        TRY(profile_events(ctx, false, &ev, err));
-        HIP_TRY(tkh_launch_paged_rows(&p, (int)dtype, D, ctx->stream, ev ? ev[0] : nullptr, ev ? ev[1] : nullptr), "paged attention launch");
-        return after_operator(ctx, err);
-    }
     // A batch may have both kinds of sequences: each kernel passes the other's by.
-    p.decode_rows = 16;
-    if (p.group <= 16) TRY(launch_decode(ctx, p, dtype, D, err));
-    if ((int64_t)p.b.max_queries * p.group > 16) TRY(launch_chunk(ctx, p, dtype, D, err));
+    p.decode_rows = dtype == TKH_F32 ? INT32_MAX : 16;
+    if (dtype == TKH_F32 || p.group <= 16) TRY(launch_decode(ctx, p, dtype, D, err));
+    if (dtype != TKH_F32 && (int64_t)p.b.max_queries * p.group > 16) TRY(launch_chunk(ctx, p, dtype, D, err));
     return after_operator(ctx, err);
 }
 
