@@ -127,7 +127,11 @@ uint32_t launch_decode(tkh_context *ctx, tkh::PagedAttend p, tkh_dtype dtype, in
     if (row_blocks > 65535) return unsupported("paged batch size", err);
     // The rows that there can be, not what every sequence might have.
     const int64_t likely = std::min<int64_t>(units, p.hkv * (((int64_t)p.b.total * p.group + p.rows - 1) / p.rows + p.b.sequences));
-    plan_splits(ctx, p, units, ctx->paged_decode_groups * units / likely, 16, ctx->paged_decode_blocks,
+    // Four workgroups a CU (64 sequences of 512 to 8192 keys: 197 us; 202 at two, 194 at
+    // eight; 4 of 100,000: 305, 302 and 320 us); two of 32 rows, whose partials are larger
+    // (4 chunks of 128 FP32 tokens: 51 us, 63 at four).
+    const int64_t groups = p.rows > 16 ? (ctx->paged_decode_groups + 1) / 2 : ctx->paged_decode_groups;
+    plan_splits(ctx, p, units, groups * units / likely, 16, ctx->paged_decode_blocks,
                 units > kPagedCounters ? 1 : tkh::PAGED_PAIRS_MAX / p.rows, D);
     hipEvent_t *ev = nullptr;
     TRY(profile_events(ctx, false, &ev, err));
