@@ -44,6 +44,29 @@ template <int DT> __device__ __forceinline__ float add_pair(uint32_t w, float su
         return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), __builtin_bit_cast(f16x2, 0x3c003c00u), sum, false);
 }
 
+// x times c in the accumulator registers.  (As plain C++, the product would live in
+// vector registers, and 256 features' O with it: copied over and back in every step.)
+// The pauses are the ones that a matrix instruction before needs until its result may be
+// read, and one behind until what was written may be; the compiler does not see into
+// asm to set them.
+__device__ __forceinline__ void scale_acc(f32x16 &x, float c) {
+    for (int i = 0; i < 16; i += 4) {
+        float a0 = x[i], a1 = x[i + 1], a2 = x[i + 2], a3 = x[i + 3], t0, t1, t2, t3;
+        asm volatile("s_nop 15\n\ts_nop 15\n\t"
+                     "v_accvgpr_read_b32 %4, %0\n\tv_accvgpr_read_b32 %5, %1\n\t"
+                     "v_accvgpr_read_b32 %6, %2\n\tv_accvgpr_read_b32 %7, %3\n\ts_nop 7\n\t"
+                     "v_mul_f32_e32 %4, %8, %4\n\tv_mul_f32_e32 %5, %8, %5\n\t"
+                     "v_mul_f32_e32 %6, %8, %6\n\tv_mul_f32_e32 %7, %8, %7\n\ts_nop 7\n\t"
+                     "v_accvgpr_write_b32 %0, %4\n\tv_accvgpr_write_b32 %1, %5\n\t"
+                     "v_accvgpr_write_b32 %2, %6\n\tv_accvgpr_write_b32 %3, %7\n\ts_nop 15\n\t"
+                     : "+a"(a0), "+a"(a1), "+a"(a2), "+a"(a3), "=&v"(t0), "=&v"(t1), "=&v"(t2), "=&v"(t3)
+                     : "v"(c));
+        x[i] = a0, x[i + 1] = a1, x[i + 2] = a2, x[i + 3] = a3;
+    }
+}
+
+__device__ __forceinline__ float uniform_float(float x) { return __builtin_bit_cast(float, uniform(__builtin_bit_cast(int, x))); }
+
 constexpr float MASS_LIMIT = 0x1p15f;
 // The base of a row that has seen no key: any finite score is far above it, which
 // sends the row's first tile to the exact path; a hidden key's -inf still weighs 0.
@@ -226,12 +249,20 @@ __global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chun
     float base = BASE_NONE, l = 0.0f;
     bool bad = false;
 
-    auto in_log2 = [&](float s) { return CAP ? tanh_fast(s * p.softcap_y) * p.softcap_log2 : s * p.scale_log2; };
+    // A cap's tanh(y) = 1 - 2 / (1 + e^2y) goes into one multiply-add with what follows.
+    const float cap_k = uniform_float(2.0f * LOG2E * p.softcap_y), cap_2 = uniform_float(-2.0f * p.softcap_log2);
+    auto capped = [&](float s, float add) {
+        return __builtin_fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * cap_k) + 1.0f), cap_2, add);
+    };
+    auto in_log2 = [&](float s) { return CAP ? capped(s, p.softcap_log2) : s * p.scale_log2; };
     // A score's weight against a base; a hidden key's score is -inf.
     auto weight = [&](float s, float from) {
         float x;
-        if constexpr (CAP) x = s == NEG_INF ? NEG_INF : in_log2(s) - from;
-        else x = __builtin_fmaf(s, p.scale_log2, -from);
+        if constexpr (CAP) {
+            x = capped(s, p.softcap_log2 - from);
+            asm("" : "+v"(x));  // formed always: a branch per weight would cut the steps to pieces
+            x = s == NEG_INF ? NEG_INF : x;
+        } else x = __builtin_fmaf(s, p.scale_log2, -from);
         return __builtin_amdgcn_exp2f(x);
     };
     // LDS addresses of this lane's operands: a base and the row's permutation.
@@ -332,7 +363,12 @@ __global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chun
     auto move_base = [&](const f32x16 &s, u32x4 (&w)[2]) {
         float mx = NEG_INF;
         for (int i = 0; i < 16; ++i) {
-            mx = fmaxf(mx, (CAP && s[i] == NEG_INF) ? NEG_INF : in_log2(s[i]));
+            float x = in_log2(s[i]);
+            if constexpr (CAP) {
+                asm("" : "+v"(x));
+                x = s[i] == NEG_INF ? NEG_INF : x;
+            }
+            mx = fmaxf(mx, x);
             __builtin_amdgcn_sched_barrier(0);
         }
         float a0, a1;
@@ -341,7 +377,11 @@ __global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chun
         base = above;
         l *= c;
         for (int f = 0; f < FB; ++f) {
-            o[f] *= c;
+            if constexpr (D == 256) {
+                scale_acc(o[f], c);
+            } else {
+                o[f] *= c;
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
         float mass = 0.0f;
@@ -369,8 +409,6 @@ __global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chun
         uint32_t kx = k_turn, vx = v_turn;
         asm volatile("" : "+v"(kx), "+v"(vx));
         asm volatile("" : "+v"(now));  // in vector registers, not among the accumulators
-        if constexpr (D == 256)
-            for (int f = 0; f < FB; ++f) asm volatile("" : "+a"(o[f]));  // and O among them
         u32x4 k = k_operand(ka, kx, 0), v = v_operand(va, vx, 0);
         float mass = 0.0f, top = 0.0f, x0 = 0.0f, x1 = 0.0f;
         auto pack = [&](int j) {  // the pair that the slot before weighed
