@@ -1023,11 +1023,11 @@ void init_tuning(tkh_context *ctx, int device) {
     ctx->prefill16_groups = std::max(1, env_int("TKH_PREFILL16_GROUPS", 64));
     ctx->prefill16_waves = env_int("TKH_PREFILL16_WAVES", 4) == 8 ? 8 : 4;
     ctx->tile_groups = std::max(1, env_int("TKH_TILE_GROUPS", 2 * ctx->cus));
-    ctx->paged_decode_groups = std::max(1, env_int("TKH_PAGED_DECODE_GROUPS", 4 * ctx->cus));
+    ctx->paged_decode_groups = std::max(1, env_int("TKH_PAGED_DECODE_GROUPS", 6 * ctx->cus));
     ctx->paged_wide_groups = std::max(1, env_int("TKH_PAGED_WIDE_GROUPS", ctx->cus));
     ctx->paged_chunk_groups = std::max(1, env_int("TKH_PAGED_CHUNK_GROUPS", 2 * ctx->cus));
     ctx->paged_chunk_tiles = std::max(1, env_int("TKH_PAGED_CHUNK_TILES", 8));
-    ctx->paged_decode_blocks = std::max(1, env_int("TKH_PAGED_DECODE_BLOCKS", 32));
+    ctx->paged_decode_blocks = std::max(1, env_int("TKH_PAGED_DECODE_BLOCKS", 16));
 }
 
 // First visible key (absolute) of a query at `position` (window_attention.rs:105-107).

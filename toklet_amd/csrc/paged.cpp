@@ -11,13 +11,11 @@
 #include "host.hpp"
 #include "paged.hpp"
 
-extern "C" hipError_t tkh_launch_paged_decode(const tkh::PagedAttend *p, int dtype, int d, int row_blocks, hipStream_t stream,
+extern "C" hipError_t tkh_launch_paged_decode(const tkh::PagedAttend *p, int dtype, int d, int groups, hipStream_t stream,
                                               hipEvent_t start, hipEvent_t stop);
 extern "C" int tkh_paged_chunk_waves(int d);
-extern "C" hipError_t tkh_launch_paged_chunk(const tkh::PagedAttend *p, int dtype, int d, int waves, int row_blocks,
+extern "C" hipError_t tkh_launch_paged_chunk(const tkh::PagedAttend *p, int dtype, int d, int waves, int groups,
                                              hipStream_t stream, hipEvent_t start, hipEvent_t stop);
-extern "C" hipError_t tkh_launch_paged_chunk_merge(const tkh::PagedAttend *p, int dtype, int d, int waves, int row_blocks,
-                                                   hipStream_t stream, hipEvent_t start, hipEvent_t stop);
 extern "C" hipError_t tkh_launch_paged_produce(const tkh::PagedProduce *p, int src, int dst, hipStream_t stream);
 extern "C" hipError_t tkh_launch_copy_pages(const tkh::CopyPages *c, hipStream_t stream);
 extern "C" hipError_t tkh_launch_patch_words(const tkh::PatchWords *w, hipStream_t stream);
@@ -91,30 +89,46 @@ uint32_t check_batch(const tkh_paged_batch &b, const tkh_paged_layout &l, tkh_er
 tkh::PagedBatch device_batch(const tkh_paged_batch &b) {
     return tkh::PagedBatch{b.page_table, b.key_lens, b.query_start, b.slots, (int64_t)b.table_stride,
                            (int32_t)b.table_rows, (int32_t)b.sequences, (int32_t)b.max_queries,
-                           (int32_t)b.max_keys, (int32_t)b.total_queries};
+                           (int32_t)b.max_keys, (int32_t)b.total_queries, 0};
 }
 tkh::PagedLayout device_layout(const tkh_paged_layout &l) {
     return tkh::PagedLayout{(int64_t)l.page_stride, (int64_t)l.head_stride, (int64_t)l.row_stride, (int32_t)l.pages,
                             __builtin_ctzll(l.page_tokens)};
 }
 
-// Key splits of a launch of `units` (sequence, KV head, row block) triples whose
-// partials hold p.rows rows: at least min_blocks blocks of `block` keys each, about
-// `target` workgroups if every sequence were as long as the longest, and at most
-// `most` (and what the workspace holds).
-void plan_splits(const tkh_context *ctx, tkh::PagedAttend &p, int64_t units, int64_t target, int64_t block,
-                 int64_t min_blocks, int64_t most, int D) {
-    const int64_t span = std::min<int64_t>(p.b.max_keys, (int64_t)p.window + p.b.max_queries);
-    const int64_t blocks = (span + block - 1) / block + 1;
-    const int64_t slot_bytes = (int64_t)p.rows * (D + 2) * sizeof(float);
-    int64_t splits = std::min<int64_t>(target / units, blocks / min_blocks);
-    splits = std::min<int64_t>(splits, ((int64_t)split_region_bytes(ctx) - 64) / slot_bytes / units);
-    splits = std::max<int64_t>(1, std::min<int64_t>(splits, most));
-    p.splits = (int32_t)splits;
-    p.split_blocks = (int32_t)((blocks + splits - 1) / splits);
+// The launches of a batch's attention, PAGED_LIST_MAX sequences each.  The kernels count
+// the work on the device; a launch has the most workgroups that there can be.  row_blocks:
+// blocks of `rows` packed rows that `sequences` sequences can have per KV head; `groups`:
+// workgroups to split their keys towards, in parts of `min_blocks` blocks of `block` keys.
+struct Splits {
+    int64_t rows, block, min_blocks, groups, most, waves;
+};
+template <class RowBlocks, class Launch>
+uint32_t launch_listed(tkh_context *ctx, tkh::PagedAttend p, int D, const Splits &sp, RowBlocks row_blocks, Launch launch, tkh_error *err) {
+    // Partials: two slots per group that is split towards, and a counter for each and wave.
+    const int64_t slot_bytes = (int64_t)p.rows * (D + 2) * sizeof(float), region = (int64_t)split_region_bytes(ctx) - 64;
+    int64_t groups = std::min<int64_t>(sp.groups, std::min<int64_t>(region / slot_bytes, kPagedCounters / sp.waves) / 2);
+    p.splits = (int32_t)(groups < 1 ? 1 : sp.most);
+    groups = std::max<int64_t>(1, groups);
+    p.min_blocks = (int32_t)sp.min_blocks;
+    p.groups = (int32_t)groups;
     p.part_ml = reinterpret_cast<float *>(ctx->workspace);
-    p.part_o = p.part_ml + (units * splits * p.rows * 2 + 3) / 4 * 4;
+    p.part_o = p.part_ml + (2 * groups * p.rows * 2 + 3) / 4 * 4;
     p.counters = ctx->paged_counters;
+    // Keys that a row block sees: window and as many more as it has tokens.
+    const int64_t tokens = std::min<int64_t>(p.b.max_queries, (sp.rows - 2) / p.group + 2);
+    const int64_t blocks = (std::min<int64_t>(p.b.max_keys, (int64_t)p.window + tokens - 1) + sp.block - 1) / sp.block;
+    const int64_t parts = std::min<int64_t>(p.splits, std::max<int64_t>(1, (blocks + sp.min_blocks - 1) / sp.min_blocks));
+    const int32_t sequences = p.b.sequences;
+    for (p.b.first = 0; p.b.first < sequences; p.b.first += tkh::PAGED_LIST_MAX) {
+        p.b.sequences = std::min(sequences - p.b.first, tkh::PAGED_LIST_MAX);
+        const int64_t units = p.hkv * row_blocks(p.b.sequences), grid = parts == 1 ? units : std::min(units * parts, units + groups);
+        if (grid > INT32_MAX / (64 * sp.waves)) return unsupported("paged batch size", err);
+        hipEvent_t *ev = nullptr;
+        TRY(profile_events(ctx, false, &ev, err));
+        HIP_TRY(launch(p, (int)grid, ev ? ev[0] : nullptr, ev ? ev[1] : nullptr), "paged attention launch");
+    }
+    return TKH_OK;
 }
 
 // paged_decode: sequences of at most 16 packed rows; with FP32 storage, all.
@@ -123,43 +137,45 @@ uint32_t launch_decode(tkh_context *ctx, tkh::PagedAttend p, tkh_dtype dtype, in
     // Up to 16 rows a block, so that a batch of single tokens stores partials of its own
     // rows only; more rows (FP32 storage) in blocks of 32.
     p.rows = (int32_t)(most <= 16 ? most : 32);
-    const int64_t row_blocks = (most + p.rows - 1) / p.rows, units = (int64_t)p.b.sequences * p.hkv * row_blocks;
-    if (row_blocks > 65535) return unsupported("paged batch size", err);
-    // The rows that there can be, not what every sequence might have.
-    const int64_t likely = std::min<int64_t>(units, p.hkv * (((int64_t)p.b.total * p.group + p.rows - 1) / p.rows + p.b.sequences));
-    // Four workgroups a CU (64 sequences of 512 to 8192 keys: 197 us; 202 at two, 194 at
-    // eight; 4 of 100,000: 305, 302 and 320 us); two of 32 rows, whose partials are larger
-    // (4 chunks of 128 FP32 tokens: 51 us, 63 at four).
-    const int64_t groups = p.rows > 16 ? (ctx->paged_decode_groups + 1) / 2 : ctx->paged_decode_groups;
-    plan_splits(ctx, p, units, groups * units / likely, 16, ctx->paged_decode_blocks,
-                units > kPagedCounters ? 1 : tkh::PAGED_PAIRS_MAX / p.rows, D);
-    hipEvent_t *ev = nullptr;
-    TRY(profile_events(ctx, false, &ev, err));
-    HIP_TRY(tkh_launch_paged_decode(&p, (int)dtype, D, (int)row_blocks, ctx->stream, ev ? ev[0] : nullptr, ev ? ev[1] : nullptr),
-            "paged decode launch");
-    return TKH_OK;
+    // Six workgroups a CU, of the two or more that it holds at once, so that they even out
+    // (64 sequences of 512 to 8192 keys: 196 us, 209 at four; 4 of 100,000: 313 and 307 us);
+    // two of 32 rows, whose partials are larger (4 chunks of 128 FP32 tokens: 48 us, 57 at
+    // three).  A split has 16 blocks at least: 24 sequences of 203 to 4096 keys, 64 to 256
+    // features, 15 to 26 us; 17 to 32 at 8 blocks as at 32.
+    Splits sp{};
+    sp.rows = p.rows > 16 ? 32 : 16;
+    sp.block = 16;
+    sp.min_blocks = ctx->paged_decode_blocks;
+    sp.groups = p.rows > 16 ? (ctx->paged_decode_groups + 2) / 3 : ctx->paged_decode_groups;
+    sp.most = tkh::PAGED_PAIRS_MAX / p.rows;
+    sp.waves = 1;
+    const int64_t all = (int64_t)p.b.total * p.group / sp.rows;
+    auto row_blocks = [&](int64_t sequences) { return p.rows > 16 ? std::min(all + sequences, sequences * ((most + 31) / 32)) : sequences; };
+    return launch_listed(ctx, p, D, sp, row_blocks, [&](const tkh::PagedAttend &a, int groups, hipEvent_t start, hipEvent_t stop) {
+        return tkh_launch_paged_decode(&a, (int)dtype, D, groups, ctx->stream, start, stop);
+    }, err);
 }
 
-// Sequences of more: the chunk kernel, and where keys are split the merge.
+// Sequences of more: the chunk kernel.
 uint32_t launch_chunk(tkh_context *ctx, tkh::PagedAttend p, tkh_dtype dtype, int D, tkh_error *err) {
-    const int64_t rows_each = (int64_t)p.b.max_queries * p.group, units = (int64_t)p.b.sequences * p.hkv;
     // Eight waves where workgroups of 256 rows still fill the CUs.
     int waves = tkh_paged_chunk_waves(D);
     if (waves == 8 && p.hkv * ((int64_t)p.b.total * p.group / 256) < ctx->paged_wide_groups) waves = 4;
-    const int64_t rows = 32 * waves, row_blocks = (rows_each + rows - 1) / rows;
-    if (units * row_blocks * 64 > INT32_MAX) return unsupported("paged batch size", err);
-    p.rows = (int32_t)rows;
-    // The rows that there can be, not what every sequence might have.
-    const int64_t likely = std::max<int64_t>(1, p.hkv * (((int64_t)p.b.total * p.group + rows - 1) / rows));
-    plan_splits(ctx, p, units * row_blocks, ctx->paged_chunk_groups * units * row_blocks / likely, 32, ctx->paged_chunk_tiles, 32, D);
-    hipEvent_t *ev = nullptr;
-    TRY(profile_events(ctx, p.splits > 1, &ev, err));
-    HIP_TRY(tkh_launch_paged_chunk(&p, (int)dtype, D, waves, (int)row_blocks, ctx->stream, ev ? ev[0] : nullptr, ev ? ev[1] : nullptr),
-            "paged chunk launch");
-    if (p.splits > 1)
-        HIP_TRY(tkh_launch_paged_chunk_merge(&p, (int)dtype, D, waves, (int)row_blocks, ctx->stream, ev ? ev[2] : nullptr, ev ? ev[3] : nullptr),
-                "paged merge launch");
-    return TKH_OK;
+    Splits sp{};
+    sp.rows = 32 * waves;
+    sp.block = 32;
+    sp.min_blocks = ctx->paged_chunk_tiles;
+    // Workgroups that the CUs hold at once: more would wait for them (24 sequences of 1 to
+    // 200 tokens, 256 features: 113 us in 256, 144 in 512).
+    sp.groups = waves == 8 || D == 256 ? (ctx->paged_chunk_groups + 1) / 2 : ctx->paged_chunk_groups;
+    sp.most = 32;
+    sp.waves = waves;
+    p.rows = (int32_t)sp.rows;
+    const int64_t all = (int64_t)p.b.total * p.group / sp.rows, most = ((int64_t)p.b.max_queries * p.group + sp.rows - 1) / sp.rows;
+    auto row_blocks = [&](int64_t sequences) { return std::min(all + sequences, sequences * most); };
+    return launch_listed(ctx, p, D, sp, row_blocks, [&](const tkh::PagedAttend &a, int groups, hipEvent_t start, hipEvent_t stop) {
+        return tkh_launch_paged_chunk(&a, (int)dtype, D, waves, groups, ctx->stream, start, stop);
+    }, err);
 }
 
 // A captured replay would repeat a launch but not the host's bookkeeping.
@@ -228,6 +244,7 @@ uint32_t tkh_paged_attention(tkh_context *ctx, const tkh_paged_batch *batch, con
     if (!std::isfinite(scale) || scale <= 0.0f) return invalid("attention scale", err);
     if (!std::isfinite(softcap) || softcap < 0.0f) return invalid("score softcap", err);
     TRY(product(batch->total_queries, query_heads, &rows, err));
+    if (rows > (1u << 30)) return unsupported("paged batch size", err);  // packed rows are 32-bit in the kernels
     TRY(product(rows, layout->head_dim, &n, err));
     TRY(length("q", q_len, n, err));
     TRY(length("context", context_len, n, err));

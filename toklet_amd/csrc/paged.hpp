@@ -5,8 +5,8 @@
 // r * row_stride + d.  Key j of a sequence is row j % page_tokens of page
 // table[j / page_tokens].  Tables, lengths and query ranges are device arrays
 // that a captured launch reads anew at each replay, so the kernels check every
-// value that becomes an address: a sequence that fails is skipped and
-// ST_BAD_PAGE raised.
+// value that becomes an address: a value that fails raises ST_BAD_PAGE, and
+// nothing is read or written through it.
 #pragma once
 
 #include "device.hpp"
@@ -20,7 +20,10 @@ struct PagedBatch {
     const int32_t *slots;        // [sequences] table rows, or null: row b
     int64_t table_stride;
     int32_t table_rows, sequences, max_queries, max_keys, total;
+    int32_t first;  // the launch's sequences are first .. first + sequences - 1 of the arrays
 };
+// Sequences that one attention launch lists; a larger batch takes several launches.
+constexpr int PAGED_LIST_MAX = 1024;
 
 struct PagedLayout {
     int64_t page_stride, head_stride, row_stride;  // elements
@@ -40,12 +43,13 @@ struct PagedAttend {
     int32_t window;   // at most 2^30, which hides no key
     float scale_log2;
     float softcap_y, softcap_log2;  // scale / cap and cap * log2(e); 0: no cap
-    int32_t splits;        // most key splits of a (sequence, KV head, row block)
-    int32_t split_blocks;  // key blocks (16 keys; 32 for chunks) a split has at least
-    int32_t decode_rows;   // sequences of at most this many packed rows are paged_decode's, others the chunk kernel's
-    int32_t rows;          // packed rows (tokens x group) a partial holds
+    int32_t splits;      // most key splits of a row block
+    int32_t min_blocks;  // key blocks (16 keys; 32 for chunks) of a split at least
+    int32_t groups;      // workgroups that the batch's key blocks are split towards
+    int32_t decode_rows;  // sequences of at most this many packed rows are paged_decode's, others the chunk kernel's
+    int32_t rows;         // packed rows (tokens x group) a partial holds
     float *part_ml, *part_o;  // [slot, rows, 2] and [slot, rows, D]
-    uint32_t *counters;       // per (sequence, KV head, row block): splits that have arrived
+    uint32_t *counters;       // at a row block's first slot: splits that have arrived
     uint32_t *status;
 };
 
@@ -98,9 +102,10 @@ struct PagedSeq {
     int32_t q0, n, len, slot;
     bool bad;
 };
-// The loads are scalar, and independent of one another as far as they can be: a
-// workgroup waits for them before anything else.
-__device__ __forceinline__ PagedSeq paged_sequence(const PagedBatch &b, int s) {
+// The loads are independent of one another as far as they can be: a workgroup waits
+// for them before anything else.
+__device__ __forceinline__ PagedSeq paged_sequence(const PagedBatch &b, int in_launch) {
+    const int s = b.first + in_launch;
     PagedSeq r;
     int32_t q1;
     if (b.query_start) {

@@ -65,15 +65,13 @@ __global__ __launch_bounds__((64 * DecodeRing<DT, D>::W)) void paged_decode(Page
     __shared__ uint32_t lds_last;
     lds_ptr<uint8_t> lds = (lds_ptr<uint8_t>)lds_mem;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, n = lane & 15;
-    const int kvh = (int)(blockIdx.x % (uint32_t)p.hkv), split = (int)(blockIdx.x / (uint32_t)p.hkv), G = p.group;
-    const PagedSeq sq = paged_sequence(p.b, blockIdx.y);
-    if (sq.bad) {
-        raise_status(p.status, true, ST_BAD_PAGE);
-        return;
-    }
+    const int G = p.group;
+    PagedWork work;
+    if (!paged_work<ROWS, 4, false>(p, (int)blockIdx.x, work)) return;
+    const PagedSeq &sq = work.sq;
+    const int kvh = work.kvh, split = work.part;
     const int all_rows = uniform(sq.n * G), pos0 = uniform(sq.len - sq.n), len = uniform(sq.len);
-    const int row0 = (int)blockIdx.z * ROWS;
-    if (all_rows > p.decode_rows || row0 >= all_rows) return;
+    const int row0 = work.rb * ROWS;
     const int nrows = all_rows - row0 < ROWS ? all_rows - row0 : ROWS;
     const int tok0 = row0 / G, tok1 = (row0 + nrows - 1) / G;  // tokens of the first and the last row
 
@@ -82,8 +80,7 @@ __global__ __launch_bounds__((64 * DecodeRing<DT, D>::W)) void paged_decode(Page
     const int see_lo = pos0 + tok0 - p.window + 1 > 0 ? pos0 + tok0 - p.window + 1 : 0, see_hi = pos0 + tok1 + 1;
     const int b_first = see_lo >> 4, b_end = see_hi > 0 ? (see_hi + 15) >> 4 : 0;
     const int blocks = b_end > b_first ? b_end - b_first : 0;
-    int active = (blocks + p.split_blocks - 1) / p.split_blocks;
-    active = active < 1 ? 1 : (active > p.splits ? p.splits : active);
+    const int active = work.active(blocks);
     if (split >= active) return;
     const int per = (blocks + active - 1) / active;
     const int b_lo = uniform(b_first + split * per);
@@ -257,7 +254,7 @@ __global__ __launch_bounds__((64 * DecodeRing<DT, D>::W)) void paged_decode(Page
     raise_status(p.status, bad_page, ST_BAD_PAGE);
     raise_status(p.status, bad, ST_NONFINITE_INPUT);
     __syncthreads();
-    const int64_t unit = ((int64_t)blockIdx.y * gridDim.z + blockIdx.z) * p.hkv + kvh, slot = unit * p.splits + split;
+    const int64_t slot0 = work.slot, slot = slot0 + split;
     const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(p.part_o + slot * p.rows * D, 0, 0x7FFFFFFF, 0x00020000);
     bool bad_out = false;
     auto finish = [&](int r, int d, f32x4 o, float mass) {
@@ -296,9 +293,9 @@ __global__ __launch_bounds__((64 * DecodeRing<DT, D>::W)) void paged_decode(Page
         wait_loads<0>();
         __syncthreads();  // every thread's stores come before the count
         if (threadIdx.x == 0) {
-            const uint32_t old = __hip_atomic_fetch_add(p.counters + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const uint32_t old = __hip_atomic_fetch_add(p.counters + slot0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             lds_last = old == (uint32_t)active - 1 ? 1u : 0u;
-            if (lds_last) __hip_atomic_store(p.counters + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (lds_last) __hip_atomic_store(p.counters + slot0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
         __syncthreads();
         if (!lds_last) return;
@@ -306,7 +303,7 @@ __global__ __launch_bounds__((64 * DecodeRing<DT, D>::W)) void paged_decode(Page
         // features of a row over its share of the splits, several loads under way.
         lds_ptr<f32x2> ml = (lds_ptr<f32x2>)lds;
         const int pairs = nrows * active, items = nrows * (D / 4);
-        const float *part_ml = p.part_ml + unit * p.splits * p.rows * 2, *part_o = p.part_o + unit * p.splits * p.rows * D;
+        const float *part_ml = p.part_ml + slot0 * p.rows * 2, *part_o = p.part_o + slot0 * p.rows * D;
         for (int i = threadIdx.x; i < pairs; i += 64 * W) {
             const int s = i / nrows, r = i % nrows;
             ml[i] = f32x2{shared_load(part_ml + (s * p.rows + r) * 2), shared_load(part_ml + (s * p.rows + r) * 2 + 1)};
@@ -359,10 +356,10 @@ __global__ __launch_bounds__((64 * DecodeRing<DT, D>::W)) void paged_decode(Page
 
 }  // namespace tkh
 
-extern "C" hipError_t tkh_launch_paged_decode(const tkh::PagedAttend *p, int dtype, int d, int row_blocks, hipStream_t stream,
+extern "C" hipError_t tkh_launch_paged_decode(const tkh::PagedAttend *p, int dtype, int d, int groups, hipStream_t stream,
                                               hipEvent_t start, hipEvent_t stop) {
     using namespace tkh;
-    const dim3 grid((unsigned)(p->hkv * p->splits), (unsigned)p->b.sequences, (unsigned)row_blocks);
+    const dim3 grid((unsigned)groups);
     auto go = [&](auto kernel, int waves) {
         hipExtLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, stream, start, stop, 0, *p);
         return hipGetLastError();

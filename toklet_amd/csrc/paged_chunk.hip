@@ -106,25 +106,8 @@ template <int D, int W> struct ChunkRing {
     static constexpr int v_plain(int f) { return (4 * f & ~bits) << 4; }
 };
 
-// The tiles of row block `rb` that one of its rows sees, and how many splits share them.
-struct ChunkSpan {
-    int t_first, t_end, active;
-};
-template <int ROWS> __device__ __forceinline__ ChunkSpan chunk_span(const PagedAttend &p, const PagedSeq &sq, int rb) {
-    const int G = p.group, pos0 = sq.len - sq.n, nrows = sq.n * G;
-    const int r0 = rb * ROWS, r1 = (r0 + ROWS < nrows ? r0 + ROWS : nrows) - 1;
-    const int lo = pos0 + r0 / G - p.window + 1, hi = pos0 + r1 / G + 1;
-    ChunkSpan s;
-    s.t_first = (lo > 0 ? lo : 0) >> 5;
-    s.t_end = hi > 0 ? (hi + 31) >> 5 : 0;
-    if (s.t_end < s.t_first) s.t_end = s.t_first;
-    s.active = (s.t_end - s.t_first + p.split_blocks - 1) / p.split_blocks;
-    s.active = s.active < 1 ? 1 : (s.active > p.splits ? p.splits : s.active);
-    return s;
-}
-
 template <int DT, int D, int W, bool CAP>
-__global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chunk(PagedAttend p, int row_blocks) {
+__global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chunk(PagedAttend p) {
     using L = ChunkRing<D, W>;
     constexpr int KT = L::KT, NS = L::NS, TG = L::TG, ROWS = 32 * W, QS = D / 16, FB = D / 32;
     __shared__ __attribute__((aligned(1024))) uint8_t lds_mem[L::bytes];
@@ -132,39 +115,24 @@ __global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chun
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
     const int G = p.group;
 
-    // Workgroups reach the XCDs in turn.  Where there are units (sequence, KV head)
-    // enough, each XCD takes a contiguous range of them, whose row blocks share K and V
-    // in its L2; a few are dealt out one by one, or some XCDs would have more work.  A
-    // unit's longest row blocks come first.
-    int unit, rb, split;
-    {
-        const uint32_t nb = gridDim.x, b = blockIdx.x, splits = (uint32_t)p.splits, units = (uint32_t)(p.b.sequences * p.hkv);
-        uint32_t rest;
-        if (units % 8 == 0 || units >= 32) {
-            const uint32_t x = b % 8, k = b / 8, per = (nb + 7) / 8, full = nb % 8 == 0 ? 8 : nb % 8;
-            const uint32_t t = x < full ? x * per + k : full * per + (x - full) * (per - 1) + k;
-            unit = (int)(t / splits / (uint32_t)row_blocks);
-            rest = t % (splits * (uint32_t)row_blocks);
-        } else {
-            unit = (int)(b % units);
-            rest = b / units;
-        }
-        split = (int)(rest % splits);
-        rb = row_blocks - 1 - (int)(rest / splits);
-    }
-    const int kvh = unit % p.hkv;
-    const PagedSeq sq = paged_sequence(p.b, unit / p.hkv);
-    if (sq.bad) {
-        raise_status(p.status, true, ST_BAD_PAGE);
-        return;
-    }
+    PagedWork work;
+    if (!paged_work<ROWS, 5, true>(p, (int)blockIdx.x, work)) return;
+    const PagedSeq &sq = work.sq;
+    const int kvh = work.kvh, rb = work.rb, split = work.part;
     const int nrows = uniform(sq.n * G), pos0 = uniform(sq.len - sq.n), len = uniform(sq.len);
-    if (nrows <= p.decode_rows || rb * ROWS >= nrows) return;
-    const ChunkSpan span = chunk_span<ROWS>(p, sq, rb);
-    if (split >= span.active) return;
-    const int per = (span.t_end - span.t_first + span.active - 1) / span.active;
-    const int t_lo = uniform(span.t_first + split * per);
-    const int t_hi = t_lo + per < span.t_end ? t_lo + per : span.t_end;
+    // The tiles that a row of the block sees, and this split's share of them.
+    int t_lo, t_hi, active;
+    {
+        const int r1 = (rb * ROWS + ROWS < nrows ? rb * ROWS + ROWS : nrows) - 1;
+        const int lo = pos0 + rb * ROWS / G - p.window + 1, hi = pos0 + r1 / G + 1;
+        const int t_first = (lo > 0 ? lo : 0) >> 5, t_end = hi > 0 ? (hi + 31) >> 5 : 0;
+        const int all = t_end > t_first ? t_end - t_first : 0;
+        active = uniform(work.active(all));
+        if (split >= active) return;
+        const int per = (all + active - 1) / active;
+        t_lo = uniform(t_first + split * per);
+        t_hi = t_lo + per < t_first + all ? t_lo + per : t_first + all;
+    }
     const int tiles = uniform(t_hi > t_lo ? t_hi - t_lo : 0);
 
     const int groups = (tiles + TG - 1) / TG;
@@ -479,82 +447,73 @@ __global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chun
         }
     }
 
-    bool bad_out = false;
-    const int64_t slot = ((int64_t)unit * row_blocks + rb) * p.splits + split;
-    float a0, a1;
-    swap_pair(l, true, a0, a1);
-    const float mass = a0 + a1;
-    int r = wave * 32 + n;  // row in the block
-    asm volatile("" : "+v"(r));  // formed again here: nothing of it lives through the loop
-    if (rb * ROWS + r < nrows) {
-        const int tok = (rb * ROWS + r) / G, head = kvh * G + (rb * ROWS + r) % G;
-        if (span.active == 1) {
-            const float inv = 1.0f / mass;
-            for (int f = 0; f < FB; ++f)
-                for (int i = 0; i < 4; ++i) {
-                    f32x4 y = {};
-                    if (pos0 + tok >= 0)
-                        for (int j = 0; j < 4; ++j) {
-                            y[j] = o[f][4 * i + j] * inv;
-                            bad_out |= !is_finite_f(y[j]);
-                        }
-                    store_elem4<DT>(p.out, ((int64_t)(sq.q0 + tok) * p.hq + head) * D + 32 * f + 8 * i + 4 * h, y);
-                }
-        } else {
-            for (int f = 0; f < FB; ++f)
-                for (int i = 0; i < 4; ++i) {
-                    const f32x4 y = {o[f][4 * i], o[f][4 * i + 1], o[f][4 * i + 2], o[f][4 * i + 3]};
-                    *gstore_ptr<f32x4>(p.part_o + (slot * ROWS + r) * D + 32 * f + 8 * i + 4 * h) = y;
-                }
-            if (h == 0) *gstore_ptr<f32x2>(p.part_ml + (slot * ROWS + r) * 2) = f32x2{base, mass};
-        }
-    }
     raise_status(p.status, bad_page, ST_BAD_PAGE);
     raise_status(p.status, bad, ST_NONFINITE_INPUT);
-    raise_status(p.status, bad_out, ST_NONFINITE_OUTPUT);
-}
-
-// The splits of every row block joined: a thread per four features of a row.
-template <int DT, int D, int ROWS>
-__global__ __launch_bounds__(256) void paged_chunk_merge(PagedAttend p, int row_blocks) {
-    constexpr int PER = 256 / (D / 4);
-    const int piece = blockIdx.x % (ROWS / PER), rb = blockIdx.x / (ROWS / PER) % row_blocks, unit = blockIdx.x / (ROWS / PER) / row_blocks;
-    const int kvh = unit % p.hkv, G = p.group;
-    const PagedSeq sq = paged_sequence(p.b, unit / p.hkv);
-    const int nrows = sq.n * G, r = piece * PER + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
-    if (sq.bad || nrows <= p.decode_rows || rb * ROWS + r >= nrows) return;
-    const ChunkSpan span = chunk_span<ROWS>(p, sq, rb);
-    if (span.active == 1) return;
-    const int64_t slot = ((int64_t)unit * row_blocks + rb) * p.splits;
-    float M = BASE_NONE, mass = 0.0f;
-    f32x4 o = {};
-    constexpr int U = 4;
-    for (int s0 = 0; s0 < span.active; s0 += U) {
-        f32x2 ml[U];
-        f32x4 part[U];
-        for (int u = 0; u < U; ++u) {
-            const int s = s0 + u < span.active ? s0 + u : span.active - 1;
-            ml[u] = *gload_ptr<f32x2>(p.part_ml + ((slot + s) * ROWS + r) * 2);
-            part[u] = *gload_ptr<f32x4>(p.part_o + ((slot + s) * ROWS + r) * D + d);
+    if (!works) return;
+    float a0, a1;
+    swap_pair(l, true, a0, a1);
+    float mass = a0 + a1;
+    int r = wave * 32 + n;  // row in the block
+    asm volatile("" : "+v"(r));  // formed again here: nothing of it lives through the loop
+    // Splits: a wave's partial as its registers have it, so that a lane reads back what the
+    // same lane of another split stored.  Each wave counts the splits that have arrived;
+    // the last one adds all of them up in split order, so the result does not depend on
+    // who is last, and leaves the counter at 0.
+    if (active > 1) {
+        const int64_t slot0 = work.slot, wave_floats = 32 * D;
+        auto part = [&](int s) { return __builtin_amdgcn_make_buffer_rsrc(p.part_o + ((slot0 + s) * W + wave) * wave_floats, 0, 0x7FFFFFFF, 0x00020000); };
+        auto pair = [&](int s) { return p.part_ml + (((slot0 + s) * W + wave) * 32 + n) * 2; };
+        {
+            const __amdgpu_buffer_rsrc_t to = part(split);
+            for (int f = 0; f < FB; ++f)
+                for (int i = 0; i < 4; ++i)
+                    __builtin_amdgcn_raw_buffer_store_b128(
+                        __builtin_bit_cast(u32x4, f32x4{o[f][4 * i], o[f][4 * i + 1], o[f][4 * i + 2], o[f][4 * i + 3]}), to,
+                        (uint32_t)lane * 16u + (uint32_t)(4 * f + i) * 1024u, 0, CPOL_SC1);
         }
-        for (int u = 0; u < U; ++u)
-            if (s0 + u < span.active) {
-                const float m = fmaxf(M, ml[u][0]), c0 = __builtin_amdgcn_exp2f(M - m), c1 = __builtin_amdgcn_exp2f(ml[u][0] - m);
-                M = m;
-                mass = c0 * mass + c1 * ml[u][1];
-                for (int j = 0; j < 4; ++j) o[j] = c0 * o[j] + c1 * part[u][j];
+        if (h == 0) {
+            shared_store(pair(split), base);
+            shared_store(pair(split) + 1, mass);
+        }
+        wait_loads<0>();
+        uint32_t *const counter = p.counters + slot0 * W + wave;
+        uint32_t old = 0;
+        if (lane == 0) old = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (uniform((int)old) != active - 1) return;
+        asm volatile("" ::: "memory");  // the loads come after the count
+        if (lane == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        float top = BASE_NONE;
+        for (int s = 0; s < active; ++s) top = fmaxf(top, shared_load(pair(s)));
+        mass = 0.0f;
+        for (int f = 0; f < FB; ++f) o[f] = f32x16{};
+        for (int s = 0; s < active; ++s) {
+            const float c = __builtin_amdgcn_exp2f(shared_load(pair(s)) - top);
+            mass = __builtin_fmaf(c, shared_load(pair(s) + 1), mass);
+            const __amdgpu_buffer_rsrc_t from = part(s);
+            for (int f = 0; f < FB; ++f) {
+                f32x4 x[4];
+                for (int i = 0; i < 4; ++i)
+                    x[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, (uint32_t)lane * 16u + (uint32_t)(4 * f + i) * 1024u, 0, CPOL_SC1));
+                for (int i = 0; i < 16; ++i) o[f][i] = __builtin_fmaf(c, x[i >> 2][i & 3], o[f][i]);
+            }
+        }
+    }
+    bool bad_out = false;
+    if (rb * ROWS + r < nrows) {
+        const int tok = (rb * ROWS + r) / G, head = kvh * G + (rb * ROWS + r) % G;
+        const float inv = 1.0f / mass;
+        for (int f = 0; f < FB; ++f)
+            for (int i = 0; i < 4; ++i) {
+                f32x4 y = {};
+                if (pos0 + tok >= 0)
+                    for (int j = 0; j < 4; ++j) {
+                        y[j] = o[f][4 * i + j] * inv;
+                        bad_out |= !is_finite_f(y[j]);
+                    }
+                store_elem4<DT>(p.out, ((int64_t)(sq.q0 + tok) * p.hq + head) * D + 32 * f + 8 * i + 4 * h, y);
             }
     }
-    const int tok = (rb * ROWS + r) / G, head = kvh * G + (rb * ROWS + r) % G;
-    bool bad = false;
-    f32x4 y = {};
-    if (sq.len - sq.n + tok >= 0)
-        for (int j = 0; j < 4; ++j) {
-            y[j] = o[j] / mass;
-            bad |= !is_finite_f(y[j]);
-        }
-    store_elem4<DT>(p.out, ((int64_t)(sq.q0 + tok) * p.hq + head) * D + d, y);
-    raise_status(p.status, bad, ST_NONFINITE_OUTPUT);
+    raise_status(p.status, bad_out, ST_NONFINITE_OUTPUT);
 }
 
 }  // namespace tkh
@@ -587,24 +546,12 @@ template <class F> hipError_t chunk_build(int dtype, int d, int waves, bool cap,
 // Most waves of a chunk workgroup, 32 rows each (it has these or 4).
 extern "C" int tkh_paged_chunk_waves(int d) { return d <= 128 ? 8 : 4; }
 
-extern "C" hipError_t tkh_launch_paged_chunk(const tkh::PagedAttend *p, int dtype, int d, int waves, int row_blocks,
+extern "C" hipError_t tkh_launch_paged_chunk(const tkh::PagedAttend *p, int dtype, int d, int waves, int groups,
                                              hipStream_t stream, hipEvent_t start, hipEvent_t stop) {
-    const int64_t groups = (int64_t)p->b.sequences * p->hkv * row_blocks * p->splits;
     return chunk_build(dtype, d, waves, p->softcap_y != 0.0f, [&](auto dt, auto dims, auto w, auto cap) {
         constexpr int W = decltype(w)::value;
         hipExtLaunchKernelGGL((tkh::paged_chunk<decltype(dt)::value, decltype(dims)::value, W, decltype(cap)::value>),
-                              dim3((unsigned)groups), dim3(64 * W), 0, stream, start, stop, 0, *p, row_blocks);
-        return hipGetLastError();
-    });
-}
-
-extern "C" hipError_t tkh_launch_paged_chunk_merge(const tkh::PagedAttend *p, int dtype, int d, int waves, int row_blocks,
-                                                   hipStream_t stream, hipEvent_t start, hipEvent_t stop) {
-    return chunk_build(dtype, d, waves, false, [&](auto dt, auto dims, auto w, auto) {
-        constexpr int D = decltype(dims)::value, ROWS = 32 * decltype(w)::value, PER = 256 / (D / 4);
-        const int64_t groups = (int64_t)p->b.sequences * p->hkv * row_blocks * (ROWS / PER);
-        hipExtLaunchKernelGGL((tkh::paged_chunk_merge<decltype(dt)::value, D, ROWS>), dim3((unsigned)groups), dim3(256), 0, stream,
-                              start, stop, 0, *p, row_blocks);
+                              dim3((unsigned)groups), dim3(64 * W), 0, stream, start, stop, 0, *p);
         return hipGetLastError();
     });
 }

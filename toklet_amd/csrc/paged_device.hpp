@@ -111,6 +111,123 @@ constexpr int CPOL_SC1 = 16;  // a buffer load past the L2, as shared_load
 // LDS for that many (maximum, mass) pairs.
 __device__ constexpr int pairs_bytes(int pairs) { return (pairs * 8 + 15) / 16 * 16; }
 
+// One workgroup's work: keys of one row block (ROWS packed rows) of a sequence and KV head.
+struct PagedWork {
+    PagedSeq sq;
+    int kvh, rb;
+    int part, parts;  // this split, and the most that a row block of the sequence has
+    int blocks;       // key blocks for which a row block has one more split
+    int slot;         // of the row block's first partial
+
+    // Splits of a row block that sees `n` key blocks.
+    __device__ int active(int n) const {
+        const int a = (n + blocks - 1) / blocks;
+        return a < 1 ? 1 : (a < parts ? a : parts);
+    }
+};
+// Workgroup `item`'s work, from the batch's lengths on the device: a ragged batch launches
+// few idle workgroups, and its keys are split by their sum, not by the longest sequence's.
+// C key blocks over R row blocks are split towards P = groups - R workgroups (half of
+// `groups` at least): a row block has a split per C / P of its blocks.  That makes fewer
+// than P + R workgroups, so no more than `groups`, which the CUs hold a whole number of times
+// (one more, and all wait for it: 4 sequences of 100,000 keys in 1024 workgroups 305 us,
+// in 1056 368 us), unless there are more row blocks than half of that; and fewer than 2 P of
+// row blocks that are split, which have partials.  Every wave works this out, a lane per
+// sequence: 0.3 us for 64.  Neighbours are of different KV heads, which go to different
+// XCDs: with eight heads (or a multiple) a head's row blocks share one L2, and each XCD
+// works on every sequence.  (Whole sequences per XCD have 2% less time where all are
+// alike, 32 chunks of 128 tokens: 326 instead of 333 us, and 30% more where they are
+// not, 24 of 1 to 200 tokens.)  Long row blocks come first.
+// MANY: the sequences of more than decode_rows packed rows; otherwise those of at most
+// that.  False: no work, or a bad batch, of which nothing is worked on.
+template <int ROWS, int SHIFT, bool MANY>
+__device__ __forceinline__ bool paged_work(const PagedAttend &p, int item, PagedWork &w) {
+    static_assert(ROWS >= 2);
+    const int lane = threadIdx.x & 63, G = p.group, S = p.b.sequences, each = (S + 63) / 64;
+    struct Need {
+        int row_blocks, blocks;  // of each KV head; keys of each
+    };
+    auto need = [&](const PagedSeq &q) {
+        const int rows = q.n * G, most = (ROWS - 2) / G + 2, tokens = q.n < most ? q.n : most;
+        const int span = p.window + tokens - 1, keys = q.len < span ? q.len : span;
+        const bool here = MANY ? rows > p.decode_rows : rows > 0 && rows <= p.decode_rows;
+        return Need{here ? (rows + ROWS - 1) / ROWS : 0, keys > 0 ? (keys + (1 << SHIFT) - 1) >> SHIFT : 1};
+    };
+    PagedSeq mine{};
+    double load = 0.0, units = 0.0;
+    bool bad = false;
+    for (int j = 0; j < each; ++j)
+        if (lane * each + j < S) {
+            const PagedSeq q = paged_sequence(p.b, lane * each + j);
+            const Need n = need(q);
+            if (j == 0) mine = q;
+            bad |= q.bad;
+            units += n.row_blocks;
+            load += (double)n.row_blocks * n.blocks;
+        }
+    raise_status(p.status, bad, ST_BAD_PAGE);
+    if (__ballot(bad) != 0) return false;
+    for (int d = 1; d < 64 && d < S; d *= 2) {
+        load += __shfl_xor(load, d);
+        units += __shfl_xor(units, d);
+    }
+    const double left = p.groups - units * p.hkv, half = 0.5 * p.groups;
+    const double share = load * p.hkv / (left > half ? left : half);
+    int blocks = uniform(share < 0x1p30 ? (int)share + 1 : 1 << 30);
+    blocks = blocks > p.min_blocks ? blocks : p.min_blocks;
+
+    struct Count {
+        int parts, items;
+    };
+    auto count = [&](const Need &n) {
+        int parts = (n.blocks + blocks - 1) / blocks;
+        parts = parts < p.splits ? parts : p.splits;
+        return Count{parts, p.hkv * n.row_blocks * parts};
+    };
+    int items = 0, slots = 0;
+    for (int j = 0; j < each; ++j)
+        if (lane * each + j < S) {
+            const Count c = count(need(j == 0 ? mine : paged_sequence(p.b, lane * each + j)));
+            items += c.items;
+            slots += c.parts > 1 ? c.items : 0;
+        }
+    int items_to = items, slots_to = slots;  // up to this lane's and with them
+    for (int d = 1; d < 64 && d < S; d *= 2) {
+        const int a = __shfl_up(items_to, d), b = __shfl_up(slots_to, d);
+        if (lane >= d) {
+            items_to += a;
+            slots_to += b;
+        }
+    }
+    const uint64_t owner = __ballot(item >= items_to - items && item < items_to);
+    if (owner == 0) return false;
+    const int o = __builtin_ctzll(owner);
+    int at = item - __builtin_amdgcn_readlane(items_to - items, o), slot = __builtin_amdgcn_readlane(slots_to - slots, o);
+    w.sq.q0 = __builtin_amdgcn_readlane(mine.q0, o);
+    w.sq.n = __builtin_amdgcn_readlane(mine.n, o);
+    w.sq.len = __builtin_amdgcn_readlane(mine.len, o);
+    w.sq.slot = __builtin_amdgcn_readlane(mine.slot, o);
+    w.sq.bad = false;
+    Need n = need(w.sq);
+    Count c = count(n);
+    for (int s = o * each + 1; at >= c.items; ++s) {  // the owner's later sequences
+        at -= c.items;
+        slot += c.parts > 1 ? c.items : 0;
+        w.sq = paged_sequence(p.b, uniform(s));
+        n = need(w.sq);
+        c = count(n);
+    }
+    at = uniform(at);
+    const int row_blocks = uniform(n.row_blocks), rest = at / p.hkv;
+    w.parts = uniform(c.parts);
+    w.blocks = blocks;
+    w.kvh = uniform(at % p.hkv);
+    w.part = uniform(rest % w.parts);
+    w.rb = uniform(row_blocks - 1 - rest / w.parts);
+    w.slot = uniform(slot + (w.kvh * row_blocks + w.rb) * w.parts);
+    return true;
+}
+
 // How far a score may pass the row's maximum before the maximum moves, in log2.
 constexpr float SLACK = 8.0f;
 
