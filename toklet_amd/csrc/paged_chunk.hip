@@ -46,19 +46,22 @@ template <int DT> __device__ __forceinline__ float add_pair(uint32_t w, float su
 
 // x times c in the accumulator registers.  (As plain C++, the product would live in
 // vector registers, and 256 features' O with it: copied over and back in every step.)
-// The pauses are the ones that a matrix instruction before needs until its result may be
-// read, and one behind until what was written may be; the compiler does not see into
-// asm to set them.
+// acc_pause comes before and behind: the compiler does not see into asm to wait until a
+// matrix instruction's result may be read, or what was written may be used by one.
+__device__ __forceinline__ void acc_pause() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15\n\ts_nop 15");
+    __builtin_amdgcn_sched_barrier(0);
+}
 __device__ __forceinline__ void scale_acc(f32x16 &x, float c) {
     for (int i = 0; i < 16; i += 4) {
         float a0 = x[i], a1 = x[i + 1], a2 = x[i + 2], a3 = x[i + 3], t0, t1, t2, t3;
-        asm volatile("s_nop 15\n\ts_nop 15\n\t"
-                     "v_accvgpr_read_b32 %4, %0\n\tv_accvgpr_read_b32 %5, %1\n\t"
-                     "v_accvgpr_read_b32 %6, %2\n\tv_accvgpr_read_b32 %7, %3\n\ts_nop 7\n\t"
+        asm volatile("v_accvgpr_read_b32 %4, %0\n\tv_accvgpr_read_b32 %5, %1\n\t"
+                     "v_accvgpr_read_b32 %6, %2\n\tv_accvgpr_read_b32 %7, %3\n\ts_nop 0\n\t"
                      "v_mul_f32_e32 %4, %8, %4\n\tv_mul_f32_e32 %5, %8, %5\n\t"
-                     "v_mul_f32_e32 %6, %8, %6\n\tv_mul_f32_e32 %7, %8, %7\n\ts_nop 7\n\t"
+                     "v_mul_f32_e32 %6, %8, %6\n\tv_mul_f32_e32 %7, %8, %7\n\ts_nop 0\n\t"
                      "v_accvgpr_write_b32 %0, %4\n\tv_accvgpr_write_b32 %1, %5\n\t"
-                     "v_accvgpr_write_b32 %2, %6\n\tv_accvgpr_write_b32 %3, %7\n\ts_nop 15\n\t"
+                     "v_accvgpr_write_b32 %2, %6\n\tv_accvgpr_write_b32 %3, %7"
                      : "+a"(a0), "+a"(a1), "+a"(a2), "+a"(a3), "=&v"(t0), "=&v"(t1), "=&v"(t2), "=&v"(t3)
                      : "v"(c));
         x[i] = a0, x[i + 1] = a1, x[i + 2] = a2, x[i + 3] = a3;
@@ -342,16 +345,18 @@ __global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chun
         float a0, a1;
         swap_pair(mx, true, a0, a1);
         const float above = fmaxf(base, fmaxf(a0, a1)), c = __builtin_amdgcn_exp2f(base - above);
-        base = above;
         l *= c;
-        for (int f = 0; f < FB; ++f) {
-            if constexpr (D == 256) {
-                scale_acc(o[f], c);
-            } else {
+        if constexpr (D == 256) {
+            acc_pause();
+            for (int f = 0; f < FB; ++f) scale_acc(o[f], c);
+            acc_pause();
+        } else if (__ballot(l != 0.0f) != 0) {  // nothing summed yet in a wave's first tile
+            for (int f = 0; f < FB; ++f) {
                 o[f] *= c;
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
         }
+        base = above;
         float mass = 0.0f;
         for (int j = 0; j < 8; ++j) {
             const uint32_t both = pack2<DT>(weight(s[2 * j], above), weight(s[2 * j + 1], above));
