@@ -146,7 +146,9 @@ uint32_t launch_decode(tkh_context *ctx, tkh::PagedAttend p, tkh_dtype dtype, in
     sp.rows = p.rows > 16 ? 32 : 16;
     sp.block = 16;
     sp.min_blocks = ctx->paged_decode_blocks;
-    sp.groups = p.rows > 16 ? (ctx->paged_decode_groups + 2) / 3 : ctx->paged_decode_groups;
+    // Two, too, where the batch may be all chunks: idle workgroups take 5 us then.
+    const bool chunks = dtype != TKH_F32 && (int64_t)p.b.max_queries * p.group > 16;
+    sp.groups = p.rows > 16 || chunks ? (ctx->paged_decode_groups + 2) / 3 : ctx->paged_decode_groups;
     sp.most = tkh::PAGED_PAIRS_MAX / p.rows;
     sp.waves = 1;
     const int64_t all = (int64_t)p.b.total * p.group / sp.rows;
