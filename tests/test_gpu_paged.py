@@ -162,6 +162,122 @@ def attention_shifted(p, skip):
     return want, tol
 
 
+def tuned(monkeypatch, stream=None, synchronous=True, **env):
+    """A context whose launches split as the settings say."""
+    from toklet_amd import ops
+
+    for name, value in env.items():
+        monkeypatch.setenv("TKH_PAGED_" + name, str(value))
+    ctx = ops.Context(0, stream=stream, synchronous=synchronous)
+    for name in env:
+        monkeypatch.delenv("TKH_PAGED_" + name)
+    return ctx
+
+
+FINEST = dict(DECODE_BLOCKS=1, DECODE_GROUPS=4096, CHUNK_TILES=1, CHUNK_GROUPS=4096)
+
+
+@pytest.mark.parametrize("window,softcap", [(None, 0.0), (500, 20.0)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_attention_many_splits(monkeypatch, dtype, d, window, softcap):
+    """As many splits as there are key blocks, of which the last to arrive joins all in one
+    order: equal results from call to call, and counters left as they were."""
+    import torch
+
+    from paged_util import Paged
+
+    ctx = tuned(monkeypatch, **FINEST)
+    for name, spans in (("decode", [(3000, 1), (129, 1), (1, 1), (0, 0), (2000, 1)]),
+                        ("chunk", [(2100, 70), (300, 33), (64, 64), (1500, 1), (20, 20)])):
+        p = Paged(spans, HEADS[d], dtype, page=16, seed=d + 1)
+        log(f"splits {name} {dtype} {d}")
+        got, want, tol = attend(ctx, p, window, softcap)
+        check(f"{name} {dtype} {d}", got, want, tol)
+        for _ in range(3):
+            assert torch.equal(attend(ctx, p, window, softcap)[0], got)
+    ctx.close()
+
+
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("window,softcap", [(None, 0.0), (100, 0.0), (33, 30.0)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_attention_wide_rows(monkeypatch, dtype, d, window, softcap, split):
+    """Workgroups of 256 rows, which large batches have, at sizes that end inside them."""
+    from paged_util import Paged
+
+    ctx = tuned(monkeypatch, WIDE_GROUPS=1, **(FINEST if split else {}))
+    for spans in ([(900, 300), (64, 64), (257, 257), (700, 5), (90, 1)], [(128, 128), (0, 0), (1060, 65)]):
+        p = Paged(spans, (8, 2, d), dtype, page=32, seed=d)
+        want = attend_with_freed_pages(p, window)
+        log(f"wide {dtype} {d} {window} {split}")
+        got, ref, tol = attend(ctx, p, window, softcap)
+        assert want
+        check(f"wide {dtype} {d} {window} {split}", got, ref, tol)
+    ctx.close()
+
+
+@pytest.mark.parametrize("sequences", [63, 64, 65, 130, 1030, 2100])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attention_many_sequences(ctx, dtype, sequences):
+    """More sequences than a wave has lanes, than one launch lists; short ones among long ones."""
+    from paged_util import Paged
+
+    spans = [(i % 37, min(i % 37, i % 4)) for i in range(sequences)]
+    spans[sequences // 2], spans[-1], spans[3] = (3000, 1), (700, 40), (1500, 33)
+    p = Paged(spans, (4, 2, 64), dtype, page=16, seed=sequences, slots=sequences % 2 == 0)
+    log(f"sequences {sequences} {dtype}")
+    check(f"{sequences} {dtype}", *attend(ctx, p))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attention_far_pages(ctx, dtype):
+    """Pages further apart than 32 bits of bytes, and of elements, reach."""
+    import torch
+
+    from paged_util import Paged
+
+    for spans in ([(90, 1), (60, 1)], [(90, 40), (60, 60)]):
+        p = Paged(spans, HEADS[64], dtype, page=16, seed=8)
+        apart = 1 << 29  # elements; 13 pages
+        store = torch.empty(2 * (p.pages - 1) * apart + 2 * 16 * 64 * 2, dtype=p.k.dtype, device="cuda")
+        k, v = (torch.as_strided(store, p.k.shape, (2 * apart, 16 * 64, 64, 1), i * 16 * 64 * 2) for i in range(2))
+        k.copy_(p.k)
+        v.copy_(p.v)
+        p.k, p.v = k, v
+        assert (p.pages - 1) * 2 * apart > 1 << 32
+        log(f"far {dtype} {spans}")
+        check(f"far {dtype}", *attend(ctx, p))
+        del k, v, store, p
+
+
+def test_attention_two_streams(monkeypatch):
+    """Two contexts on streams of their own, at work at the same time, give what each gives alone."""
+    import torch
+
+    from paged_util import Paged
+    from toklet_amd import ops
+
+    work = []
+    for i in range(2):
+        ctx = tuned(monkeypatch, stream=torch.cuda.Stream(), **FINEST)
+        p = Paged([(2500 - 900 * i, 1), (900, 40 + i), (33, 33)], HEADS[128], "bf16", page=16, seed=i)
+        torch.cuda.synchronize()
+        alone, out = torch.empty_like(p.q), torch.empty_like(p.q)
+        ops.paged_attention(ctx, p.batch(), p.q, p.k, p.v, alone, scale=0.1)
+        ctx.close()
+        work.append((tuned(monkeypatch, stream=torch.cuda.Stream(), synchronous=False, **FINEST), p, p.batch(), alone, out))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for ctx, p, batch, _, out in work:
+            ops.paged_attention(ctx, batch, p.q, p.k, p.v, out, scale=0.1)
+    for ctx, _, _, alone, out in work:
+        ctx.synchronize()
+        assert torch.equal(out, alone)
+        ctx.close()
+
+
 def test_attention_large_scores(ctx):
     """Scores of hundreds, one key far above the others, and equal scores."""
     import torch
@@ -315,15 +431,13 @@ def produced(ctx, p, rot, norm, fused, proj, eps=1e-6):
     assert torch.equal(k0.nan_to_num(3.0), p.k.nan_to_num(3.0)) and torch.equal(v0.nan_to_num(3.0), p.v.nan_to_num(3.0))
 
 
-@pytest.mark.parametrize("layout", ["none", "half", "interleaved"])
-@pytest.mark.parametrize("scaling", ["none", "linear", "bands"])
+@pytest.mark.parametrize("layout,scaling", [("none", "none"), ("half", "none"), ("half", "linear"), ("half", "bands"),
+                                            ("interleaved", "none"), ("interleaved", "linear"), ("interleaved", "bands")])
 @pytest.mark.parametrize("dtype,proj", [("bf16", "f32"), ("f16", "f16"), ("f32", "f32"), ("bf16", "bf16"), ("f32", "bf16")])
 def test_produce(ctx, layout, scaling, dtype, proj):
     from paged_util import Paged
     from toklet_amd import ops
 
-    if layout == "none" and scaling != "none":
-        pytest.skip("no rotation to scale")
     for d, r in ((64, 0), (64, 8), (128, 0), (128, 64), (128, 120), (256, 0), (256, 40)):
         p = Paged([(1, 1), (0, 0), (49, 33), (2000, 1), (17, 16)], HEADS[d], dtype, page=16, seed=d + r, slots=r == 64,
                   token_major=r == 8, spare=2)
@@ -531,4 +645,39 @@ def test_captured_steps():
             ctx.synchronize()
             assert torch.equal(out, eager), i
     kv.close()
+    ctx.close()
+
+
+def test_captured_chunks(monkeypatch):
+    """A captured pass of chunks and single tokens with split keys, replayed with eager passes in between."""
+    import torch
+
+    from paged_util import Paged
+    from toklet_amd import ops
+
+    stream = torch.cuda.Stream()
+    ctx = tuned(monkeypatch, stream=stream, synchronous=False, **FINEST)
+    p = Paged([(1400, 40), (700, 1), (0, 0), (200, 200)], HEADS[128], "bf16", page=16, seed=3)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        out, eager = torch.empty_like(p.q), torch.empty_like(p.q)
+        batch = p.batch()
+
+        def step(to):
+            ops.paged_attention(ctx, batch, p.q, p.k, p.v, to, scale=0.1)
+
+        step(eager)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step(out)
+        for i in range(6):
+            p.q.copy_(torch.randn_like(p.q))
+            if i == 3:  # lengths that the replay reads anew
+                p.lens[p.rows[0]] = 1300
+            out.fill_(0.0)
+            graph.replay()
+            step(eager)
+            ctx.synchronize()
+            assert torch.equal(out, eager), i
     ctx.close()
