@@ -208,6 +208,11 @@ def test_attention_refusals():
         rc, err = attention(lay=layout(**kw), kv=10 ** 6)
         assert rc == _lib.INVALID_PARAMETER and err.tensor == b"context", kw
     assert attention(lay=layout(page_stride=2 ** 62))[0] == _lib.SIZE_OVERFLOW
+    # Strides whose bytes pass 32 bits, and more query rows than 2^30.
+    for kw in (dict(page_stride=2 ** 30 + 8), dict(row_stride=2 ** 17 + 8, page_stride=2 ** 29)):
+        assert attention(lay=layout(**kw))[0] == _lib.UNSUPPORTED, kw
+    assert attention(lay=layout(pages=1, page_stride=2 ** 31))[1].tensor == b"context"
+    assert attention(batch(total_queries=2 ** 24, query_start=64), heads=128)[0] == _lib.UNSUPPORTED
     for name in ("sequences", "max_queries", "max_keys", "table_rows", "table_stride"):
         assert attention(batch(**{name: 0}))[0] == _lib.ZERO_DIMENSION, name
     assert attention(batch(total_queries=3))[0] == _lib.LENGTH

@@ -50,8 +50,6 @@ uint32_t check_layout(const tkh_paged_layout &l, uint64_t *extent, tkh_error *er
     // Rows of one page apart from each other: heads outside rows, or rows outside heads.
     if (l.row_stride < l.head_dim || (l.kv_heads > 1 && l.head_stride < l.head_dim))
         return invalid("page rows overlap", err);
-    // A page's bytes, and a row's place in it, are 32-bit in the kernels.
-    if (l.row_stride > (1u << 17) || (l.pages > 1 && l.page_stride > (1u << 30))) return unsupported("page strides", err);
     uint64_t heads, rows, span, n;
     TRY(product(l.kv_heads - 1, l.head_stride, &heads, err));
     TRY(product(l.page_tokens - 1, l.row_stride, &rows, err));
@@ -64,6 +62,8 @@ uint32_t check_layout(const tkh_paged_layout &l, uint64_t *extent, tkh_error *er
     TRY(add(n, span, extent, err));
     if (*extent > (uint64_t)INT64_MAX / 8)
         return fail(err, TKH_SIZE_OVERFLOW, nullptr, 0, 0, 0, "tensor size arithmetic overflow");
+    // A page's bytes, and a row's place in it, are 32-bit in the kernels.
+    if (l.row_stride > (1u << 17) || (l.pages > 1 && l.page_stride > (1u << 30))) return unsupported("page strides", err);
     return TKH_OK;
 }
 
