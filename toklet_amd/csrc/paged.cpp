@@ -137,18 +137,23 @@ uint32_t launch_decode(tkh_context *ctx, tkh::PagedAttend p, tkh_dtype dtype, in
     // Up to 16 rows a block, so that a batch of single tokens stores partials of its own
     // rows only; more rows (FP32 storage) in blocks of 32.
     p.rows = (int32_t)(most <= 16 ? most : 32);
-    // Six workgroups a CU, of the two or more that it holds at once, so that they even out
-    // (64 sequences of 512 to 8192 keys: 196 us, 209 at four; 4 of 100,000: 313 and 307 us);
-    // two of 32 rows, whose partials are larger (4 chunks of 128 FP32 tokens: 48 us, 57 at
-    // three).  A split has 16 blocks at least: 24 sequences of 203 to 4096 keys, 64 to 256
+    // Six workgroups a CU, of the two or more that it holds at once, so that sequences of
+    // different lengths even out (64 of 512 to 8192 keys: 190 us, 209 at four); four where
+    // there are so few sequences and KV heads that each is split evenly (4 of 100,000 keys:
+    // 307 us, 322 at six); two of 32 rows, whose partials are larger (4 chunks of 128 FP32
+    // tokens: 48 us, 57 at three), and where the batch may be all chunks, when idle
+    // workgroups only cost time (5 us of 6 a CU).
+    // A split has 16 blocks at least: 24 sequences of 203 to 4096 keys, 64 to 256
     // features, 15 to 26 us; 17 to 32 at 8 blocks as at 32.
+    const bool chunks = dtype != TKH_F32 && (int64_t)p.b.max_queries * p.group > 16;
+    int64_t groups = ctx->paged_decode_groups;
+    if (p.rows > 16 || chunks) groups = (groups + 2) / 3;
+    else if (6 * (int64_t)p.b.sequences * p.hkv < groups) groups = (2 * groups + 2) / 3;
     Splits sp{};
     sp.rows = p.rows > 16 ? 32 : 16;
     sp.block = 16;
     sp.min_blocks = ctx->paged_decode_blocks;
-    // Two, too, where the batch may be all chunks: idle workgroups take 5 us then.
-    const bool chunks = dtype != TKH_F32 && (int64_t)p.b.max_queries * p.group > 16;
-    sp.groups = p.rows > 16 || chunks ? (ctx->paged_decode_groups + 2) / 3 : ctx->paged_decode_groups;
+    sp.groups = groups;
     sp.most = tkh::PAGED_PAIRS_MAX / p.rows;
     sp.waves = 1;
     const int64_t all = (int64_t)p.b.total * p.group / sp.rows;
