@@ -44,28 +44,14 @@ template <int DT> __device__ __forceinline__ float add_pair(uint32_t w, float su
         return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), __builtin_bit_cast(f16x2, 0x3c003c00u), sum, false);
 }
 
-// x times c in the accumulator registers.  (As plain C++, the product would live in
-// vector registers, and 256 features' O with it: copied over and back in every step.)
-// acc_pause comes before and behind: the compiler does not see into asm to wait until a
-// matrix instruction's result may be read, or what was written may be used by one.
-__device__ __forceinline__ void acc_pause() {
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_nop 15\n\ts_nop 15");
-    __builtin_amdgcn_sched_barrier(0);
-}
+// x times c, from and to the accumulator registers: if O lived in vector registers on
+// this path alone, every step would copy it over and back.
 __device__ __forceinline__ void scale_acc(f32x16 &x, float c) {
-    for (int i = 0; i < 16; i += 4) {
-        float a0 = x[i], a1 = x[i + 1], a2 = x[i + 2], a3 = x[i + 3], t0, t1, t2, t3;
-        asm volatile("v_accvgpr_read_b32 %4, %0\n\tv_accvgpr_read_b32 %5, %1\n\t"
-                     "v_accvgpr_read_b32 %6, %2\n\tv_accvgpr_read_b32 %7, %3\n\ts_nop 0\n\t"
-                     "v_mul_f32_e32 %4, %8, %4\n\tv_mul_f32_e32 %5, %8, %5\n\t"
-                     "v_mul_f32_e32 %6, %8, %6\n\tv_mul_f32_e32 %7, %8, %7\n\ts_nop 0\n\t"
-                     "v_accvgpr_write_b32 %0, %4\n\tv_accvgpr_write_b32 %1, %5\n\t"
-                     "v_accvgpr_write_b32 %2, %6\n\tv_accvgpr_write_b32 %3, %7"
-                     : "+a"(a0), "+a"(a1), "+a"(a2), "+a"(a3), "=&v"(t0), "=&v"(t1), "=&v"(t2), "=&v"(t3)
-                     : "v"(c));
-        x[i] = a0, x[i + 1] = a1, x[i + 2] = a2, x[i + 3] = a3;
-    }
+    f32x16 t = x;
+    asm volatile("" : "+v"(t));
+    t *= c;
+    asm volatile("" : "+a"(t));
+    x = t;
 }
 
 __device__ __forceinline__ float uniform_float(float x) { return __builtin_bit_cast(float, uniform(__builtin_bit_cast(int, x))); }
@@ -346,15 +332,10 @@ __global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chun
         swap_pair(mx, true, a0, a1);
         const float above = fmaxf(base, fmaxf(a0, a1)), c = __builtin_amdgcn_exp2f(base - above);
         l *= c;
-        if constexpr (D == 256) {
-            acc_pause();
-            for (int f = 0; f < FB; ++f) scale_acc(o[f], c);
-            acc_pause();
-        } else if (__ballot(l != 0.0f) != 0) {  // nothing summed yet in a wave's first tile
-            for (int f = 0; f < FB; ++f) {
-                o[f] *= c;
-                __builtin_amdgcn_sched_barrier(0);
-            }
+        for (int f = 0; f < FB; ++f) {
+            if constexpr (D == 256) scale_acc(o[f], c);
+            else o[f] *= c;
+            __builtin_amdgcn_sched_barrier(0);
         }
         base = above;
         float mass = 0.0f;

@@ -154,7 +154,7 @@ __device__ __forceinline__ bool paged_work(const PagedAttend &p, int item, Paged
         return Need{here ? (rows + ROWS - 1) / ROWS : 0, keys > 0 ? (keys + (1 << SHIFT) - 1) >> SHIFT : 1};
     };
     PagedSeq mine{};
-    double load = 0.0, units = 0.0;
+    float load = 0.0f, units = 0.0f;  // each lane ends with the same sums
     bool bad = false;
     for (int j = 0; j < each; ++j)
         if (lane * each + j < S) {
@@ -162,8 +162,8 @@ __device__ __forceinline__ bool paged_work(const PagedAttend &p, int item, Paged
             const Need n = need(q);
             if (j == 0) mine = q;
             bad |= q.bad;
-            units += n.row_blocks;
-            load += (double)n.row_blocks * n.blocks;
+            units += (float)n.row_blocks;
+            load += (float)n.row_blocks * (float)n.blocks;
         }
     raise_status(p.status, bad, ST_BAD_PAGE);
     if (__ballot(bad) != 0) return false;
@@ -171,9 +171,11 @@ __device__ __forceinline__ bool paged_work(const PagedAttend &p, int item, Paged
         load += __shfl_xor(load, d);
         units += __shfl_xor(units, d);
     }
-    const double left = p.groups - units * p.hkv, half = 0.5 * p.groups;
-    const double share = load * p.hkv / (left > half ? left : half);
-    int blocks = uniform(share < 0x1p30 ? (int)share + 1 : 1 << 30);
+    // Rounded sums: P (at most 32768) splits become P (1 + 2^-17) at most, which no count of
+    // workgroups or slots, being whole, passes.
+    const float left = (float)p.groups - units * (float)p.hkv, half = 0.5f * (float)p.groups;
+    const float share = load * (float)p.hkv / (left > half ? left : half);
+    int blocks = uniform(share < 0x1p30f ? (int)share + 1 : 1 << 30);
     blocks = blocks > p.min_blocks ? blocks : p.min_blocks;
 
     struct Count {
