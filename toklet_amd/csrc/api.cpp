@@ -1027,7 +1027,7 @@ void init_tuning(tkh_context *ctx, int device) {
     ctx->paged_wide_groups = std::max(1, env_int("TKH_PAGED_WIDE_GROUPS", ctx->cus));
     ctx->paged_chunk_groups = std::max(1, env_int("TKH_PAGED_CHUNK_GROUPS", 2 * ctx->cus));
     ctx->paged_chunk_tiles = std::max(1, env_int("TKH_PAGED_CHUNK_TILES", 8));
-    ctx->paged_decode_blocks = std::max(1, env_int("TKH_PAGED_DECODE_BLOCKS", 16));
+    ctx->paged_decode_blocks = std::max(1, env_int("TKH_PAGED_DECODE_BLOCKS", 8));
 }
 
 // First visible key (absolute) of a query at `position` (window_attention.rs:105-107).

@@ -150,7 +150,7 @@ struct tkh_context {
     uint64_t split_wait_ticks = 50000000;  // bound of a decode merge's wait for its splits
     uint32_t *paged_counters = nullptr;  // kPagedCounters arrival counters, 0 between launches, in status_dev's allocation
     int paged_decode_groups = 1536;  // paged decode: workgroups to split towards (a third as many of 32 rows)
-    int paged_decode_blocks = 16;    // ... 16-key blocks per split at least
+    int paged_decode_blocks = 8;     // ... 16-key blocks per split at least
     int paged_wide_groups = 256;     // paged chunks: 256-row workgroups from which a workgroup has eight waves
     int paged_chunk_groups = 512;    // ... workgroups to split the keys towards (half as many where a CU holds one)
     int paged_chunk_tiles = 8;       // ... 32-key tiles per split at least

@@ -99,9 +99,10 @@ tkh::PagedLayout device_layout(const tkh_paged_layout &l) {
 // The launches of a batch's attention, PAGED_LIST_MAX sequences each.  The kernels count
 // the work on the device; a launch has the most workgroups that there can be.  row_blocks:
 // blocks of `rows` packed rows that `sequences` sequences can have per KV head; `groups`:
-// workgroups to split their keys towards, in parts of `min_blocks` blocks of `block` keys.
+// workgroups to split their keys towards, in parts of `min_blocks` blocks of `block` keys
+// at least.
 struct Splits {
-    int64_t rows, block, min_blocks, groups, most, waves;
+    int64_t rows, block, min_blocks, groups, groups_short, most, waves;
 };
 template <class RowBlocks, class Launch>
 uint32_t launch_listed(tkh_context *ctx, tkh::PagedAttend p, int D, const Splits &sp, RowBlocks row_blocks, Launch launch, tkh_error *err) {
@@ -112,6 +113,7 @@ uint32_t launch_listed(tkh_context *ctx, tkh::PagedAttend p, int D, const Splits
     groups = std::max<int64_t>(1, groups);
     p.min_blocks = (int32_t)sp.min_blocks;
     p.groups = (int32_t)groups;
+    p.groups_short = (int32_t)std::min(groups, sp.groups_short);
     p.part_ml = reinterpret_cast<float *>(ctx->workspace);
     p.part_o = p.part_ml + (2 * groups * p.rows * 2 + 3) / 4 * 4;
     p.counters = ctx->paged_counters;
@@ -141,10 +143,10 @@ uint32_t launch_decode(tkh_context *ctx, tkh::PagedAttend p, tkh_dtype dtype, in
     // different lengths even out (64 of 512 to 8192 keys: 190 us, 209 at four); four where
     // there are so few sequences and KV heads that each is split evenly (4 of 100,000 keys:
     // 307 us, 322 at six); two of 32 rows, whose partials are larger (4 chunks of 128 FP32
-    // tokens: 48 us, 57 at three), and where the batch may be all chunks, when idle
-    // workgroups only cost time (5 us of 6 a CU).
-    // A split has 16 blocks at least: 24 sequences of 203 to 4096 keys, 64 to 256
-    // features, 15 to 26 us; 17 to 32 at 8 blocks as at 32.
+    // tokens: 48 us, 57 at three), where the batch may be all chunks, when idle
+    // workgroups only cost time (5 us of 6 a CU), and where six would have fewer than 32
+    // blocks each (24 sequences of 203 to 4096 keys, 128 features: 18 us, 23 at six).
+    // A split has eight blocks at least: one sequence of 1000 keys 9.6 us, 11 at 16, 17 at 32.
     const bool chunks = dtype != TKH_F32 && (int64_t)p.b.max_queries * p.group > 16;
     int64_t groups = ctx->paged_decode_groups;
     if (p.rows > 16 || chunks) groups = (groups + 2) / 3;
@@ -154,6 +156,7 @@ uint32_t launch_decode(tkh_context *ctx, tkh::PagedAttend p, tkh_dtype dtype, in
     sp.block = 16;
     sp.min_blocks = ctx->paged_decode_blocks;
     sp.groups = groups;
+    sp.groups_short = (ctx->paged_decode_groups + 2) / 3;
     sp.most = tkh::PAGED_PAIRS_MAX / p.rows;
     sp.waves = 1;
     const int64_t all = (int64_t)p.b.total * p.group / sp.rows;
@@ -174,7 +177,7 @@ uint32_t launch_chunk(tkh_context *ctx, tkh::PagedAttend p, tkh_dtype dtype, int
     sp.min_blocks = ctx->paged_chunk_tiles;
     // Workgroups that the CUs hold at once: more would wait for them (24 sequences of 1 to
     // 200 tokens, 256 features: 113 us in 256, 144 in 512).
-    sp.groups = waves == 8 || D == 256 ? (ctx->paged_chunk_groups + 1) / 2 : ctx->paged_chunk_groups;
+    sp.groups = sp.groups_short = waves == 8 || D == 256 ? (ctx->paged_chunk_groups + 1) / 2 : ctx->paged_chunk_groups;
     sp.most = 32;
     sp.waves = waves;
     p.rows = (int32_t)sp.rows;

@@ -45,7 +45,7 @@ struct PagedAttend {
     float softcap_y, softcap_log2;  // scale / cap and cap * log2(e); 0: no cap
     int32_t splits;      // most key splits of a row block
     int32_t min_blocks;  // key blocks (16 keys; 32 for chunks) of a split at least
-    int32_t groups;      // workgroups that the batch's key blocks are split towards
+    int32_t groups, groups_short;  // workgroups that the batch's key blocks are split towards; if into short parts
     int32_t decode_rows;  // sequences of at most this many packed rows are paged_decode's, others the chunk kernel's
     int32_t rows;         // packed rows (tokens x group) a partial holds
     float *part_ml, *part_o;  // [slot, rows, 2] and [slot, rows, D]

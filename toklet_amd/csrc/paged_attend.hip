@@ -7,8 +7,10 @@
 //
 // paged_decode: blocks of 16 NR packed rows (tokens x query heads of one KV head); for
 // 16-bit storage one block of 16, and more rows are the chunk kernel's, for FP32
-// storage any number.  Bound by the bytes of K and V with few rows, by the FP32 matrix
-// instructions (1/16 of the 16-bit ones' rate) with many.
+// storage any number.  Bound by the bytes of K and V with few rows (4 sequences of 100,000
+// to 131,000 keys 307 us, 6.5 TB/s; 64 of 512 to 8192 keys 190 us, 5.9 TB/s; a copy of
+// 2 GiB reads and writes 4.85), by the FP32 matrix instructions (1/16 of the 16-bit
+// ones' rate) with many (4 chunks of 128 tokens, 14/2 heads of 64, 49 us, 53 TFLOP/s).
 //  * The keys are cut into blocks of 16, which never leave a page, and a
 //    workgroup takes one split of them.  Its waves take blocks in turn, each
 //    through a ring of its own in LDS filled by direct global->LDS loads: no
@@ -186,7 +188,7 @@ __global__ __launch_bounds__((64 * DecodeRing<DT, D>::W)) void paged_decode(Page
         u32x2 pw[NR];
         for (int a = 0; a < NR; ++a) {
             float x[4];
-            for (int i = 0; i < 4; ++i) x[i] = CAP ? tanh_fast(s[a][i] * p.softcap_y) * p.softcap_log2 : s[a][i] * p.scale_log2;
+            for (int i = 0; i < 4; ++i) x[i] = CAP ? (HALF ? tanh_fast(s[a][i] * p.softcap_y) : tanh_fp32(s[a][i] * p.softcap_y)) * p.softcap_log2 : s[a][i] * p.scale_log2;
             if (inside) {
                 for (int i = 0; i < 4; ++i) bad |= !is_finite_f(s[a][i]);
             } else {

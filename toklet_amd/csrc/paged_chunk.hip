@@ -1,18 +1,27 @@
 // paged_chunk.hip - attention of chunks of new tokens over a page table, 16-bit
-// storage: many query rows per KV head, bound by the matrix cores.
+// storage: many query rows per KV head, bound by the matrix instructions and by what
+// feeds them.
 //
 // A workgroup takes 128 or 256 packed rows (tokens x query heads of one KV head) of one
-// sequence, 32 to a wave.  K and V come in tiles of 32 keys
-// through a ring in LDS, filled by direct global->LDS loads whose page number is
-// uniform in a wave (a load run lies in one 16-key block, and those never leave a
-// page).
+// sequence, 32 to a wave, and all keys that they see or a split of them.  K and V come in
+// tiles of 32 keys through a ring in LDS, filled by direct global->LDS loads whose page
+// number is uniform in a wave (a load run lies in one 16-key block, and those never leave
+// a page).
 //  * S^T = K Q^T on v_mfma_f32_32x32x16, Q in registers as the B operand: lane l
 //    holds query row l % 32 and 16 keys, in the order that the B operand of
 //    O^T = V^T P^T wants, if V^T's keys are read in that order too (two transposing
 //    LDS loads per operand).  P never moves between lanes.
-//  * The scores of tile t + 1 are formed while the softmax of tile t runs.
+//  * The scores of tile t + 1 are formed while the softmax of tile t runs and the values
+//    of tile t - 1 are added: per matrix instruction six vector instructions, about as
+//    many as its time holds.
 //  * A row's exponent base is a maximum that it has seen; it moves only when a
 //    tile's mass against it passes 2^15, which 16-bit weights and FP32 sums hold.
+//  * 256 rows (eight waves, two to a SIMD) where they fill the CUs: 32 chunks of 128 tokens
+//    after 4096, 32/8 heads of 128, 328 us against 339 of 128 rows; 850 TFLOP/s.  A prompt
+//    of 8192 tokens 570 us, 965 TFLOP/s.  Without softmax the same instructions reach 1200:
+//    every operand is read from LDS for one matrix instruction, which is LDS's whole rate.
+//    (64 rows to a wave read half as much, but leave one wave to a SIMD: 720 us.)
+//  * 256 features fill the registers with one wave to a SIMD: 700 TFLOP/s.
 //  * Sequences of at most 16 packed rows are left to paged_decode.
 #include <cstddef>
 #include <type_traits>
@@ -64,8 +73,9 @@ constexpr float BASE_NONE = -0x1p100f;
 }  // namespace
 
 // The rings: NS groups of TG tiles of 32 keys of K, and as many of V, whose tiles are
-// read two steps after K's.  The waves meet once per group.  A tile is runs of 1 KiB, each RR whole rows as one direct
-// load of a wave leaves them, with a few bytes between runs; a row's 16-byte pieces
+// read two steps after K's.  The waves meet once per group.  A tile is runs of 1 KiB,
+// each RR whole rows as one direct load of a wave leaves them, with a few bytes between
+// runs; a row's 16-byte pieces
 // are permuted by its place in the run (piece c at c ^ turn).  The two together
 // spread over all banks both the 16 rows that a K read takes at one feature and the
 // four rows x 64 bytes that a transposing V read takes; and since the permutation

@@ -173,8 +173,13 @@ __device__ __forceinline__ bool paged_work(const PagedAttend &p, int item, Paged
     }
     // Rounded sums: P (at most 32768) splits become P (1 + 2^-17) at most, which no count of
     // workgroups or slots, being whole, passes.
-    const float left = (float)p.groups - units * (float)p.hkv, half = 0.5f * (float)p.groups;
-    const float share = load * (float)p.hkv / (left > half ? left : half);
+    auto split = [&](int groups) {
+        const float left = (float)groups - units * (float)p.hkv, half = 0.5f * (float)groups;
+        return load * (float)p.hkv / (left > half ? left : half);
+    };
+    float share = split(p.groups);
+    // Parts so short that their start and join would be most of them: fewer.
+    if (p.groups_short < p.groups && share < 4.0f * (float)p.min_blocks) share = split(p.groups_short);
     int blocks = uniform(share < 0x1p30f ? (int)share + 1 : 1 << 30);
     blocks = blocks > p.min_blocks ? blocks : p.min_blocks;
 
@@ -182,7 +187,8 @@ __device__ __forceinline__ bool paged_work(const PagedAttend &p, int item, Paged
         int parts, items;
     };
     auto count = [&](const Need &n) {
-        int parts = (n.blocks + blocks - 1) / blocks;
+        // A join costs what some min_blocks more do: a split in two is not worth it.
+        int parts = n.blocks <= 2 * p.min_blocks ? 1 : (n.blocks + blocks - 1) / blocks;
         parts = parts < p.splits ? parts : p.splits;
         return Count{parts, p.hkv * n.row_blocks * parts};
     };
@@ -228,6 +234,26 @@ __device__ __forceinline__ bool paged_work(const PagedAttend &p, int item, Paged
     w.rb = uniform(row_blocks - 1 - rest / w.parts);
     w.slot = uniform(slot + (w.kvh * row_blocks + w.rb) * w.parts);
     return true;
+}
+
+// tanh for FP32 scores: a cap multiplies its error, so small arguments (most, where the cap
+// is far above the scores) take the Taylor series, whose error is relative, and others
+// 1 - 2 / (1 + e^2|y|) with a refined reciprocal: 2^-22 of the result at 1/2, 2^-23 above.
+// The form of tanh_fast for all of them loses a factor of 7 (caps of 30 and 50).
+__device__ __forceinline__ float tanh_fp32(float y) {
+    const float x = y * y;
+    float p = -929569.0f / 638512875.0f;
+    p = __builtin_fmaf(p, x, 21844.0f / 6081075.0f);
+    p = __builtin_fmaf(p, x, -1382.0f / 155925.0f);
+    p = __builtin_fmaf(p, x, 62.0f / 2835.0f);
+    p = __builtin_fmaf(p, x, -17.0f / 315.0f);
+    p = __builtin_fmaf(p, x, 2.0f / 15.0f);
+    p = __builtin_fmaf(p, x, -1.0f / 3.0f);
+    const float d = __builtin_amdgcn_exp2f(2.0f * LOG2E * __builtin_fabsf(y)) + 1.0f;
+    float r = __builtin_amdgcn_rcpf(d);
+    if (d < 0x1p126f) r = __builtin_fmaf(r, __builtin_fmaf(-d, r, 1.0f), r);  // beyond, r is 0 beside 1
+    const float far = __builtin_copysignf(__builtin_fmaf(-2.0f, r, 1.0f), y);
+    return x <= 0.25f ? __builtin_fmaf(y * x, p, y) : far;
 }
 
 // How far a score may pass the row's maximum before the maximum moves, in log2.
