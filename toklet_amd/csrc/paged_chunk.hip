@@ -380,11 +380,20 @@ __global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chun
             w[j >> 2][j & 3] = both;
             mass = add_pair<DT>(both, mass);
         };
+        auto vector_work = [&](int u, int part) {  // of slot u, in two parts
+            if (part == 0) {
+                if (u > 0) pack(u - 1);
+                x0 = weight(now[2 * u], base);
+            } else {
+                top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, __builtin_fabsf(now[2 * u])), __builtin_fabsf(now[2 * u + 1]));
+                x1 = weight(now[2 * u + 1], base);
+            }
+        };
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int z = 0; z < QS / 4; ++z) {
+                __builtin_amdgcn_sched_barrier(0);
                 const int m = u * (QS / 4) + z, i = m / 2;
                 if (m % 2 == 0) {
                     o[i % FB] = mfma_32x32x16<DT>(v, before[i / FB], o[i % FB]);
@@ -393,11 +402,9 @@ __global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chun
                     next = mfma_32x32x16<DT>(k, q[i], i == 0 ? f32x16{} : next);
                     if (i + 1 < QS) k = k_operand(ka, kx, i + 1);
                 }
+                if (QS / 4 == 1 || z == QS / 8 - 1) vector_work(u, 0);
+                if (z == QS / 4 - 1) vector_work(u, 1);
             }
-            if (u > 0) pack(u - 1);
-            top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, __builtin_fabsf(now[2 * u])), __builtin_fabsf(now[2 * u + 1]));
-            x0 = weight(now[2 * u], base);
-            x1 = weight(now[2 * u + 1], base);
         }
         __builtin_amdgcn_sched_barrier(0);
         pack(7);
