@@ -330,7 +330,9 @@ uint32_t tkh_kv_reset_batch(tkh_kv *const *kvs, uint64_t count, tkh_error *err);
  * Element (head h, row r, feature d) of page g of one layer's K (or V) sits at
  * g * page_stride + h * head_stride + r * row_stride + d.  page_tokens is a
  * power of two from 16 to 1024, head_dim 64, 128 or 256; strides are multiples
- * of 8 elements, pointers of 16 bytes. */
+ * of 8 elements, pointers of 16 bytes; row_stride is at most 2^17 elements, and
+ * page_stride, where there are several pages, a page's extent to 2^30
+ * (TKH_UNSUPPORTED beyond).  Heads lie within rows or rows within heads. */
 typedef struct tkh_paged_layout {
     uint64_t pages, page_tokens, kv_heads, head_dim;
     uint64_t page_stride, head_stride, row_stride;
@@ -345,10 +347,11 @@ typedef struct tkh_paged_layout {
  * max_queries).  key_lens counts its keys, the new tokens among them: token i of
  * n sits at position key_lens - n + i.  Table entries past the last key are not
  * read.  Rows of no sequence (behind the last one) are neither read nor written.
- * A sequence whose values are out of range (a slot, a row range, more than
- * max_queries rows or max_keys keys, a page number) is reported as
- * TKH_INVALID_CONFIG at the next status check and reads and writes nothing
- * outside the buffers; results are then unspecified. */
+ * Values out of range (a slot, a row range, more than max_queries rows or max_keys
+ * keys, a page number) are reported as TKH_INVALID_CONFIG at the next status
+ * check; nothing outside the buffers is read or written, and the results of the
+ * whole call are then unspecified.  At most 65535 sequences, 2^24 rows (2^30 with
+ * their query heads), 2^30 keys. */
 typedef struct tkh_paged_batch {
     uint64_t sequences, total_queries, max_queries, max_keys;
     uint64_t table_rows, table_stride;

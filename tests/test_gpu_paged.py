@@ -636,6 +636,8 @@ def test_captured_steps():
         with torch.cuda.graph(graph, stream=stream):
             with pytest.raises(ops.TkhError):
                 kv.extend(seqs, [1, 1, 1])
+            with pytest.raises(ops.TkhError):  # its clearing would be recorded
+                paged.PagedKv(ctx, 1, hkv, d, 16, 8, 2, 4, torch.bfloat16)
             step(out)
         for i in range(6):
             kv.extend(seqs, [1, 1, 17 if i == 2 else 1])

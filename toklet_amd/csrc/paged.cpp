@@ -80,7 +80,7 @@ uint32_t check_batch(const tkh_paged_batch &b, const tkh_paged_layout &l, tkh_er
     TRY(product(b.table_stride, l.page_tokens, &n, err));
     if (b.max_keys > n) return invalid("max_keys exceeds the page table's rows", err);
     // Positions, rows and table indexes are 32-bit in the kernels.
-    if (b.total_queries > (1u << 24) || b.max_queries > (1u << 24) || b.sequences > 65535 || b.max_keys > (1u << 30) ||
+    if (b.total_queries >= (1u << 24) || b.max_queries > (1u << 24) || b.sequences > 65535 || b.max_keys > (1u << 30) ||
         b.table_rows > INT32_MAX || b.table_stride > INT32_MAX)
         return unsupported("paged batch size", err);
     return TKH_OK;
@@ -125,7 +125,7 @@ uint32_t launch_listed(tkh_context *ctx, tkh::PagedAttend p, int D, const Splits
     for (p.b.first = 0; p.b.first < sequences; p.b.first += tkh::PAGED_LIST_MAX) {
         p.b.sequences = std::min(sequences - p.b.first, tkh::PAGED_LIST_MAX);
         const int64_t units = p.hkv * row_blocks(p.b.sequences), grid = parts == 1 ? units : std::min(units * parts, units + groups);
-        if (grid > INT32_MAX / (64 * sp.waves)) return unsupported("paged batch size", err);
+        if (grid > INT32_MAX / 512) return unsupported("paged batch size", err);  // threads of a launch are 32-bit
         hipEvent_t *ev = nullptr;
         TRY(profile_events(ctx, false, &ev, err));
         HIP_TRY(launch(p, (int)grid, ev ? ev[0] : nullptr, ev ? ev[1] : nullptr), "paged attention launch");
@@ -548,6 +548,7 @@ uint32_t tkh_paged_create(tkh_context *ctx, const tkh_paged_options *options, tk
     if (planes > 65535 || words + o.sequences > (uint64_t)INT32_MAX || o.sequences > 65535 ||
         o.sequence_pages * o.page_tokens > (1u << 30) || l.page_stride * esize(o.storage) > (uint64_t)1 << 31)
         return unsupported("paged cache size", err);
+    if (ctx) TRY(not_capturing(ctx, err));
     auto *kv = new (std::nothrow) tkh_paged_kv();
     if (!kv) return device_error(hipErrorOutOfMemory, "paged cache", err);
     kv->o = o;

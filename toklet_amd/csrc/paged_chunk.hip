@@ -17,11 +17,13 @@
 //  * A row's exponent base is a maximum that it has seen; it moves only when a
 //    tile's mass against it passes 2^15, which 16-bit weights and FP32 sums hold.
 //  * 256 rows (eight waves, two to a SIMD) where they fill the CUs: 32 chunks of 128 tokens
-//    after 4096, 32/8 heads of 128, 328 us against 339 of 128 rows; 850 TFLOP/s.  A prompt
-//    of 8192 tokens 570 us, 965 TFLOP/s.  Without softmax the same instructions reach 1200:
-//    every operand is read from LDS for one matrix instruction, which is LDS's whole rate.
-//    (64 rows to a wave read half as much, but leave one wave to a SIMD: 720 us.)
-//  * 256 features fill the registers with one wave to a SIMD: 700 TFLOP/s.
+//    after 4096, 32/8 heads of 128, 326 us against 339 of 128 rows; 855 TFLOP/s.  A prompt
+//    of 8192 tokens 560 us, 980 TFLOP/s: of its cycles the matrix instructions fill 47%, the
+//    vector ones 48%, LDS 23% without a conflict; a wave waits for LDS, loads or the others
+//    in 23%.  (64 rows to a wave need half the LDS reads, but leave one wave to a SIMD with
+//    nothing to fill its waits: 720 us.)
+//  * 256 features fill the registers with one wave to a SIMD: 8 chunks of 2048 tokens of up
+//    to 4096 700 TFLOP/s.
 //  * Sequences of at most 16 packed rows are left to paged_decode.
 #include <cstddef>
 #include <type_traits>
@@ -361,7 +363,8 @@ __global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chun
     // Scores of tile t + 1, weights of tile t and values of tile t - 1 together, in eight
     // slots of QS / 4 matrix instructions and the weights of one pair of keys, which the
     // scheduler keeps in this order: the vector instructions fill the matrix
-    // instructions' time.  The first step adds values and the last forms scores of a tile
+    // instructions' time, half of a slot's behind each half of its matrix instructions (a
+    // prompt of 8192: 571 us with all behind the last).  The first step adds values and the last forms scores of a tile
     // that is not there: weights of zero against a cleared tile, and scores that nobody
     // uses.
     auto step = [&](int t, f32x16 &now, f32x16 &next, u32x4 (&w)[2], const u32x4 (&before)[2]) {
