@@ -350,7 +350,7 @@ typedef struct tkh_paged_layout {
  * Values out of range (a slot, a row range, more than max_queries rows or max_keys
  * keys, a page number) are reported as TKH_INVALID_CONFIG at the next status
  * check; nothing outside the buffers is read or written, and the results of the
- * whole call are then unspecified.  At most 65535 sequences, 2^24 rows (2^30 with
+ * whole call are then unspecified.  At most 65535 sequences, 2^24 - 1 rows (2^30 with
  * their query heads), 2^30 keys. */
 typedef struct tkh_paged_batch {
     uint64_t sequences, total_queries, max_queries, max_keys;

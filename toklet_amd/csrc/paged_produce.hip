@@ -11,6 +11,9 @@
 // t = p f_j / 2 pi, and reduced by t - rint(t), so a far position costs no
 // precision; sine and cosine are FP32 of the reduced turns, corrected by what
 // the rounding of the turns left out.
+// Bound by the bytes of the rows: 6000 tokens of 8/4 heads of 256, norms and interleaved
+// pairs, FP32 to bf16, 14.5 us, 4.7 TB/s (a copy of 2 GiB: 4.85).  One token 3.5 us, 64
+// single ones 4.4: a launch and the trips to the lengths, the table and the rows.
 #include <cstddef>
 #include <type_traits>
 
@@ -181,7 +184,9 @@ __global__ __launch_bounds__(256) void paged_produce(PagedProduce p, int rows, i
     raise_status(p.status, nonfinite, ST_NONFINITE_INPUT);
 }
 
-// Page copies: workgroup (chunk, pair, plane) moves CHUNK units of one page.
+// Page copies: workgroup (chunk, pair, plane) moves four units per thread of one page,
+// all loads before the stores.  1.6 GB in three launches 327 us, 4.95 TB/s; 24 pages of
+// 32 KiB in 56 planes 18 us, 4.8.
 constexpr int COPY_UNITS = 4;  // units per thread
 template <class T>
 __global__ __launch_bounds__(256) void copy_pages(CopyPages c) {
