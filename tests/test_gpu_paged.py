@@ -231,6 +231,22 @@ def test_attention_many_sequences(ctx, dtype, sequences):
     check(f"{sequences} {dtype}", *attend(ctx, p))
 
 
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("heads", [(8, 4, 256), (12, 3, 128), (7, 7, 64), (16, 8, 128), (9, 1, 128)])
+def test_attention_chunks_of_many(monkeypatch, heads, split):
+    """Chunks of many sequences, some of them none and some single tokens: every row block of
+    every head is worked on once, however the list is dealt out."""
+    from paged_util import Paged
+
+    ctx = tuned(monkeypatch, **(FINEST if split else {}))
+    for count in (9, 33, 61):
+        spans = [(40 + 23 * i % 300, (0, 1, 17, 40, 3)[i % 5] if i % 7 else 40) for i in range(count)]
+        p = Paged(spans, heads, "bf16", page=16, seed=count)
+        log(f"many chunks {heads} {split} {count}")
+        check(f"many chunks {heads} {split} {count}", *attend(ctx, p))
+    ctx.close()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_attention_far_pages(ctx, dtype):
     """Pages further apart than 32 bits of bytes, and of elements, reach."""

@@ -23,7 +23,7 @@
 //    in 23%.  (64 rows to a wave need half the LDS reads, but leave one wave to a SIMD with
 //    nothing to fill its waits: 720 us.)
 //  * 256 features fill the registers with one wave to a SIMD: 8 chunks of 2048 tokens of up
-//    to 4096 700 TFLOP/s.
+//    to 4096 keys 573 us, 720 TFLOP/s.
 //  * Sequences of at most 16 packed rows are left to paged_decode.
 #include <cstddef>
 #include <type_traits>
@@ -392,11 +392,14 @@ __global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chun
                 x1 = weight(now[2 * u + 1], base);
             }
         };
+        // A cap's longer chains want more room to be spread in: slots of two pairs (24 chunks of
+        // 1024 tokens, 128 features, 540 us; 590 with one).
+        constexpr int PAIRS = CAP && D == 128 ? 2 : 1, MS = PAIRS * QS / 4;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
+        for (int u = 0; u < 8; u += PAIRS) {
 #pragma unroll
-            for (int z = 0; z < QS / 4; ++z) {
-                __builtin_amdgcn_sched_barrier(0);
+            for (int z = 0; z < MS; ++z) {
+                if (PAIRS == 1 || z == 0) __builtin_amdgcn_sched_barrier(0);
                 const int m = u * (QS / 4) + z, i = m / 2;
                 if (m % 2 == 0) {
                     o[i % FB] = mfma_32x32x16<DT>(v, before[i / FB], o[i % FB]);
@@ -405,9 +408,10 @@ __global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chun
                     next = mfma_32x32x16<DT>(k, q[i], i == 0 ? f32x16{} : next);
                     if (i + 1 < QS) k = k_operand(ka, kx, i + 1);
                 }
-                if (QS / 4 == 1 || z == QS / 8 - 1) vector_work(u, 0);
-                if (z == QS / 4 - 1) vector_work(u, 1);
+                if (PAIRS == 1 && (MS == 1 || z == MS / 2 - 1)) vector_work(u, 0);
+                if (PAIRS == 1 && z == MS - 1) vector_work(u, 1);
             }
+            for (int w = 0; PAIRS == 2 && w < 4; ++w) vector_work(u + w / 2, w % 2);
         }
         __builtin_amdgcn_sched_barrier(0);
         pack(7);

@@ -133,11 +133,14 @@ struct PagedWork {
 // (one more, and all wait for it: 4 sequences of 100,000 keys in 1024 workgroups 305 us,
 // in 1056 368 us), unless there are more row blocks than half of that; and fewer than 2 P of
 // row blocks that are split, which have partials.  Every wave works this out, a lane per
-// sequence: 0.3 us for 64.  Neighbours are of different KV heads, which go to different
-// XCDs: with eight heads (or a multiple) a head's row blocks share one L2, and each XCD
-// works on every sequence.  (Whole sequences per XCD have 2% less time where all are
-// alike, 32 chunks of 128 tokens: 326 instead of 333 us, and 30% more where they are
-// not, 24 of 1 to 200 tokens.)  Long row blocks come first.
+// sequence: 0.3 us for 64.
+// Workgroups reach the XCDs in turn.  Neighbours are of different KV heads, so with eight
+// heads (or a multiple) a head's row blocks share one L2, and each XCD works on every
+// sequence; whole sequences per XCD have 2% less time where all are alike (32 chunks of 128
+// tokens) and 30% more where they are not.  With other numbers of heads, each XCD takes
+// a contiguous part of the list, head by head, if there are 32 (sequence, KV head) pairs
+// to make the parts alike: 8 chunks of 2048 tokens, 8/4 heads of 256, 573 us, 620 by
+// neighbours; fewer pairs are dealt out one by one.  Long row blocks come first.
 // MANY: the sequences of more than decode_rows packed rows; otherwise those of at most
 // that.  False: no work, or a bad batch, of which nothing is worked on.
 template <int ROWS, int SHIFT, bool MANY>
@@ -207,6 +210,13 @@ __device__ __forceinline__ bool paged_work(const PagedAttend &p, int item, Paged
             slots_to += b;
         }
     }
+    bool by_xcd = false;
+    if (MANY && p.hkv % 8 != 0 && (each > 1 || __builtin_popcountll(__ballot(items > 0)) * p.hkv >= 32)) {
+        const int all = __builtin_amdgcn_readlane(items_to, S < 64 ? S - 1 : 63), x = item % 8;
+        if (item >= all) return false;
+        item = x * (all / 8) + (x < all % 8 ? x : all % 8) + item / 8;
+        by_xcd = true;
+    }
     const uint64_t owner = __ballot(item >= items_to - items && item < items_to);
     if (owner == 0) return false;
     const int o = __builtin_ctzll(owner);
@@ -226,10 +236,11 @@ __device__ __forceinline__ bool paged_work(const PagedAttend &p, int item, Paged
         c = count(n);
     }
     at = uniform(at);
-    const int row_blocks = uniform(n.row_blocks), rest = at / p.hkv;
+    const int row_blocks = uniform(n.row_blocks), of_head = uniform(row_blocks * c.parts);
+    const int rest = by_xcd ? at % of_head : at / p.hkv;
     w.parts = uniform(c.parts);
     w.blocks = blocks;
-    w.kvh = uniform(at % p.hkv);
+    w.kvh = uniform(by_xcd ? at / of_head : at % p.hkv);
     w.part = uniform(rest % w.parts);
     w.rb = uniform(row_blocks - 1 - rest / w.parts);
     w.slot = uniform(slot + (w.kvh * row_blocks + w.rb) * w.parts);
