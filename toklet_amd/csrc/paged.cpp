@@ -276,6 +276,8 @@ uint32_t tkh_paged_attention(tkh_context *ctx, const tkh_paged_batch *batch, con
     p.hq = (int32_t)query_heads;
     p.hkv = (int32_t)layout->kv_heads;
     p.group = p.hq / p.hkv;
+    p.by_hkv = tkh::Divisor::of((uint32_t)p.hkv);
+    p.by_group = tkh::Divisor::of((uint32_t)p.group);
     p.window = window == 0 || window > (1u << 30) ? 1 << 30 : (int32_t)window;  // no key is further back
     p.scale_log2 = scale * 1.4426950408889634f;
     p.softcap_y = softcap != 0.0f ? scale / softcap : 0.0f;

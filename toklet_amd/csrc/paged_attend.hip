@@ -75,7 +75,7 @@ __global__ __launch_bounds__((64 * DecodeRing<DT, D>::W)) void paged_decode(Page
     const int all_rows = uniform(sq.n * G), pos0 = uniform(sq.len - sq.n), len = uniform(sq.len);
     const int row0 = work.rb * ROWS;
     const int nrows = all_rows - row0 < ROWS ? all_rows - row0 : ROWS;
-    const int tok0 = row0 / G, tok1 = (row0 + nrows - 1) / G;  // tokens of the first and the last row
+    const int tok0 = p.by_group(row0), tok1 = p.by_group(row0 + nrows - 1);  // tokens of the first and the last row
 
     // The blocks that some row sees, and this split's share of them.
     const int first_key = pos0 - p.window + 1 > 0 ? pos0 - p.window + 1 : 0;  // of the sequence
@@ -84,7 +84,7 @@ __global__ __launch_bounds__((64 * DecodeRing<DT, D>::W)) void paged_decode(Page
     const int blocks = b_end > b_first ? b_end - b_first : 0;
     const int active = work.active(blocks);
     if (split >= active) return;
-    const int per = (blocks + active - 1) / active;
+    const int per = active > 1 ? quotient(blocks + active - 1, active) : blocks;
     const int b_lo = uniform(b_first + split * per);
     const int b_hi = b_lo + per < b_end ? b_lo + per : b_end;
     const int mine = uniform(b_hi - b_lo > wave ? (b_hi - b_lo - wave + W - 1) / W : 0);
@@ -127,7 +127,7 @@ __global__ __launch_bounds__((64 * DecodeRing<DT, D>::W)) void paged_decode(Page
     u32x4 q[NR][QP];
     int lo[NR], hi[NR];  // visible keys [lo, hi)
     for (int a = 0; a < NR; ++a) {
-        const int rr = row0 + (16 * a + n < nrows ? 16 * a + n : nrows - 1), tok = rr / G, head = kvh * G + rr % G;
+        const int rr = row0 + (16 * a + n < nrows ? 16 * a + n : nrows - 1), tok = p.by_group(rr), head = kvh * G + rr - tok * G;
         const uint8_t *at = reinterpret_cast<const uint8_t *>(p.q) + ((int64_t)(sq.q0 + tok) * p.hq + head) * L::row;
         for (int s = 0; s < QP; ++s) q[a][s] = *gload_ptr<u32x4>(at + 16 * (HALF ? 4 * s + g : QP * g + s));
         lo[a] = pos0 + tok - p.window + 1;
@@ -260,7 +260,7 @@ __global__ __launch_bounds__((64 * DecodeRing<DT, D>::W)) void paged_decode(Page
     const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(p.part_o + slot * p.rows * D, 0, 0x7FFFFFFF, 0x00020000);
     bool bad_out = false;
     auto finish = [&](int r, int d, f32x4 o, float mass) {
-        const int tok = (row0 + r) / G, head = kvh * G + (row0 + r) % G;
+        const int tok = p.by_group(row0 + r), head = kvh * G + row0 + r - tok * G;
         f32x4 y = {};
         if (pos0 + tok >= 0)
             for (int i = 0; i < 4; ++i) {

@@ -125,12 +125,12 @@ __global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chun
     int t_lo, t_hi, active;
     {
         const int r1 = (rb * ROWS + ROWS < nrows ? rb * ROWS + ROWS : nrows) - 1;
-        const int lo = pos0 + rb * ROWS / G - p.window + 1, hi = pos0 + r1 / G + 1;
+        const int lo = pos0 + p.by_group(rb * ROWS) - p.window + 1, hi = pos0 + p.by_group(r1) + 1;
         const int t_first = (lo > 0 ? lo : 0) >> 5, t_end = hi > 0 ? (hi + 31) >> 5 : 0;
         const int all = t_end > t_first ? t_end - t_first : 0;
         active = uniform(work.active(all));
         if (split >= active) return;
-        const int per = (all + active - 1) / active;
+        const int per = active > 1 ? quotient(all + active - 1, active) : all;
         t_lo = uniform(t_first + split * per);
         t_hi = t_lo + per < t_first + all ? t_lo + per : t_first + all;
     }
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chun
     int pos;  // -2^30 - 1: a row past the last, which sees nothing
     {
         const int r = wave_row + n, rr = r < nrows ? r : nrows - 1;
-        const int tok = rr / G, head = kvh * G + rr % G;
+        const int tok = p.by_group(rr), head = kvh * G + rr - tok * G;
         pos = r < nrows ? pos0 + tok : -(1 << 30) - 1;
         for (int s = 0; s < QS; ++s)
             q[s] = *gload_ptr<u32x4>(reinterpret_cast<const uint16_t *>(p.q) + ((int64_t)(sq.q0 + tok) * p.hq + head) * D + 16 * s + 8 * h);
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chun
 
     const int wave_last = wave_row + 31 < nrows ? wave_row + 31 : nrows - 1;
     // Keys that every row of the wave sees: [full_lo, full_hi).
-    const int full_lo = uniform(pos0 + wave_last / G - p.window + 1), full_hi = uniform(pos0 + wave_row / G + 1);
+    const int full_lo = uniform(pos0 + p.by_group(wave_last) - p.window + 1), full_hi = uniform(pos0 + p.by_group(wave_row) + 1);
     const int first_key = pos0 - p.window + 1 > 0 ? pos0 - p.window + 1 : 0;
 
     f32x16 o[FB] = {};
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(64 * W, W == 8 || D <= 128 ? 2 : 1) void paged_chun
     }
     bool bad_out = false;
     if (rb * ROWS + r < nrows) {
-        const int tok = (rb * ROWS + r) / G, head = kvh * G + (rb * ROWS + r) % G;
+        const int tok = p.by_group(rb * ROWS + r), head = kvh * G + rb * ROWS + r - tok * G;
         const float inv = 1.0f / mass;
         for (int f = 0; f < FB; ++f)
             for (int i = 0; i < 4; ++i) {

@@ -88,11 +88,6 @@ __device__ __forceinline__ float quad_sum(float x) {
     return a + b;
 }
 
-template <int DT> __device__ __forceinline__ void store_elem(void *base, int64_t i, float x) {
-    if constexpr (DT == F32) reinterpret_cast<float *>(base)[i] = x;
-    else if constexpr (DT == F16) reinterpret_cast<_Float16 *>(base)[i] = (_Float16)x;
-    else reinterpret_cast<__bf16 *>(base)[i] = (__bf16)x;
-}
 template <int DT> __device__ __forceinline__ void store_elem4(void *base, int64_t i, f32x4 x) {
     if constexpr (DT == F32) *gstore_ptr<f32x4>(reinterpret_cast<float *>(base) + i) = x;
     else *gstore_ptr<u32x2>(reinterpret_cast<uint16_t *>(base) + i) = pack4<DT>(x);
@@ -111,6 +106,9 @@ constexpr int CPOL_SC1 = 16;  // a buffer load past the L2, as shared_load
 // LDS for that many (maximum, mass) pairs.
 __device__ constexpr int pairs_bytes(int pairs) { return (pairs * 8 + 15) / 16 * 16; }
 
+// Of numbers that are not negative.
+__device__ __forceinline__ int quotient(int a, int b) { return (int)((uint32_t)a / (uint32_t)b); }
+
 // One workgroup's work: keys of one row block (ROWS packed rows) of a sequence and KV head.
 struct PagedWork {
     PagedSeq sq;
@@ -121,7 +119,7 @@ struct PagedWork {
 
     // Splits of a row block that sees `n` key blocks.
     __device__ int active(int n) const {
-        const int a = (n + blocks - 1) / blocks;
+        const int a = quotient(n + blocks - 1, blocks);
         return a < 1 ? 1 : (a < parts ? a : parts);
     }
 };
@@ -151,7 +149,7 @@ __device__ __forceinline__ bool paged_work(const PagedAttend &p, int item, Paged
         int row_blocks, blocks;  // of each KV head; keys of each
     };
     auto need = [&](const PagedSeq &q) {
-        const int rows = q.n * G, most = (ROWS - 2) / G + 2, tokens = q.n < most ? q.n : most;
+        const int rows = q.n * G, most = p.by_group(ROWS - 2) + 2, tokens = q.n < most ? q.n : most;
         const int span = p.window + tokens - 1, keys = q.len < span ? q.len : span;
         const bool here = MANY ? rows > p.decode_rows : rows > 0 && rows <= p.decode_rows;
         return Need{here ? (rows + ROWS - 1) / ROWS : 0, keys > 0 ? (keys + (1 << SHIFT) - 1) >> SHIFT : 1};
@@ -191,7 +189,7 @@ __device__ __forceinline__ bool paged_work(const PagedAttend &p, int item, Paged
     };
     auto count = [&](const Need &n) {
         // A join costs what some min_blocks more do: a split in two is not worth it.
-        int parts = n.blocks <= 2 * p.min_blocks ? 1 : (n.blocks + blocks - 1) / blocks;
+        int parts = n.blocks <= 2 * p.min_blocks ? 1 : quotient(n.blocks + blocks - 1, blocks);
         parts = parts < p.splits ? parts : p.splits;
         return Count{parts, p.hkv * n.row_blocks * parts};
     };
@@ -228,7 +226,7 @@ __device__ __forceinline__ bool paged_work(const PagedAttend &p, int item, Paged
     w.sq.bad = false;
     Need n = need(w.sq);
     Count c = count(n);
-    for (int s = o * each + 1; at >= c.items; ++s) {  // the owner's later sequences
+    for (int s = o * each + 1; at >= c.items && s < S; ++s) {  // the owner's later sequences
         at -= c.items;
         slot += c.parts > 1 ? c.items : 0;
         w.sq = paged_sequence(p.b, uniform(s));
@@ -236,15 +234,17 @@ __device__ __forceinline__ bool paged_work(const PagedAttend &p, int item, Paged
         c = count(n);
     }
     at = uniform(at);
+    if (at >= c.items) return false;  // only if the lengths change under the launch
     const int row_blocks = uniform(n.row_blocks), of_head = uniform(row_blocks * c.parts);
-    const int rest = by_xcd ? at % of_head : at / p.hkv;
+    const int high = by_xcd ? quotient(at, of_head) : p.by_hkv(at), rest = by_xcd ? at - high * of_head : high;
     w.parts = uniform(c.parts);
     w.blocks = blocks;
-    w.kvh = uniform(by_xcd ? at / of_head : at % p.hkv);
-    w.part = uniform(rest % w.parts);
-    w.rb = uniform(row_blocks - 1 - rest / w.parts);
+    w.kvh = uniform(by_xcd ? high : at - high * p.hkv);
+    const int back = w.parts > 1 ? quotient(rest, w.parts) : rest;
+    w.part = uniform(rest - back * w.parts);
+    w.rb = uniform(row_blocks - 1 - back);
     w.slot = uniform(slot + (w.kvh * row_blocks + w.rb) * w.parts);
-    return true;
+    return w.parts == 1 || w.slot + w.parts <= 2 * p.groups;  // likewise
 }
 
 // tanh for FP32 scores: a cap multiplies its error, so small arguments (most, where the cap
